@@ -527,6 +527,75 @@ int msplat_init_gaussians(const float *xyz, const unsigned char *rgb, long long 
 int msplat_eval_metrics(const float *rendered, const float *gt, int height, int width,
                         int window_size, float sigma, float *psnr, float *ssim, float *l1);
 
+/* ---- dropout and 4-bit colours ---------------------------------------------
+ * Operators on device arrays of the current device.  No counterpart in the
+ * reference.  Each is queued on cuda_stream (NULL = the legacy default
+ * stream; pass msplat_get_stream() to run in order with the engine's calls),
+ * keeps nothing between calls, allocates nothing and does not wait, so calls
+ * may overlap, come from several threads and be captured into CUDA graphs.
+ * Arguments are checked before any CUDA call; every index is 64-bit.  No
+ * output may overlap an input, except that msplat_dropout works in place.
+ */
+
+/* Dropout: y = x / (1 - rate) where kept and 0 where dropped, for `rows` rows
+ * of `cols` floats, x_stride and y_stride floats apart (0: cols).  One draw
+ * per element, or with whole_rows != 0 one per row.  No mask is stored: draw
+ * i (row * cols + column, or the row) is word i % 4 of the Philox4x32-10 block
+ * of key `seed` and counter (i / 4, step), and drops when it is below
+ * rate * 2^32 rounded; 1 - rate above is what that threshold leaves.  So the
+ * backward pass is this call on the gradient of y with the same seed and
+ * step, and a mask is this call on ones.  A dropped value is not read as a
+ * number (a NaN there becomes 0).  0 <= rate < 1; in place (y == x) is
+ * allowed with equal strides. */
+int msplat_dropout(long long rows, int cols, const float *x, long long x_stride, float *y,
+                   long long y_stride, double rate, unsigned long long seed,
+                   unsigned long long step, int whole_rows, void *cuda_stream);
+
+/* 4-bit colour records.  The SH coefficients of one Gaussian in 8, 16, 24,
+ * 32 or 48 bytes (SH degree 0 to 4): dc as three halves, then, from degree 1
+ * on, a scale byte b for each of r, g, b (2^(b - 127), as in the OCP MX
+ * formats) and the rest coefficients as e2m1 codes (4-bit floats: 0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6 and their negatives), two to a byte, low nibble first, in
+ * the order of features_rest [B,3]; the last bytes are zero.  A channel's
+ * scale puts its largest magnitude in [3.5, 7), so that every coefficient is
+ * within half a step of the e2m1 grid; coefficients round to nearest, ties to
+ * even (from 7 * 2^125 on they saturate at 6 * 2^125).  A NaN or an infinity makes its channel of that Gaussian NaN
+ * (b = 255); dc beyond 65504 becomes infinite.  Record arrays are aligned to
+ * 16 bytes (8 at degrees 0 and 2). */
+int msplat_mx4_record_bytes(int degree);
+
+/* Records of n Gaussians from features_dc (n,3) and features_rest (n,B,3),
+ * B = (degree + 1)^2 - 1 (features_rest may be NULL at degree 0). */
+int msplat_mx4_pack(int n, int degree, const float *features_dc, const float *features_rest,
+                    void *records, void *cuda_stream);
+
+/* The values that the records stand for, exactly. */
+int msplat_mx4_unpack(int n, int degree, const void *records, float *features_dc,
+                      float *features_rest, void *cuda_stream);
+
+/* Colours of n Gaussians from num_views (0 to 64) camera positions cam_pos
+ * (num_views,3; host): colors (num_views,n,3) = the SH basis of the direction
+ * from the camera to the mean, times the coefficients; degrees up to
+ * degrees_to_use (<= degree).  The raw colour, as the rasterizer takes it
+ * (it adds 0.5 and clamps at 0).  Bit for bit what the renderer computes from the
+ * unpacked coefficients.  With radii (num_views,n; NULL: all visible) the
+ * colours of Gaussians of radius <= 0 are not written.  A mean at the camera
+ * has no direction: its colour is NaN unless degrees_to_use is 0. */
+int msplat_mx4_colors(int n, int degree, int degrees_to_use, const float *means3d,
+                      const void *records, int num_views, const float *cam_pos,
+                      const int32_t *radii, float *colors, void *cuda_stream);
+
+/* Gradient of the coefficients from v_colors (num_views,n,3), summed over the
+ * views: straight through the rounding to records, view directions taken as
+ * constants (both as the training step takes them).  Every element of
+ * v_features_dc (n,3) and v_features_rest (n,B,3) is written: 0 above the
+ * degrees in use and for Gaussians that no view sees.  v_colors is not read
+ * where radii (num_views,n; NULL: all visible) is <= 0. */
+int msplat_mx4_colors_backward(int n, int degree, int degrees_to_use, const float *means3d,
+                               int num_views, const float *cam_pos, const int32_t *radii,
+                               const float *v_colors, float *v_features_dc,
+                               float *v_features_rest, void *cuda_stream);
+
 /* ---- introspection (tests and benchmarks) ------------------------------- */
 
 /* Loss of the last step; waits for it when `sync` != 0, else returns the

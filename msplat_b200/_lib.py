@@ -179,6 +179,15 @@ SIGNATURES = {
         _i, _p, _p, _f, _p, _fp, _fp, _f, _f, _f, _f, _u, _u, _ip, _f, _u, _u, _fp,
         _p, _p, _p, _fp, _p, _p,
     ]),
+    "msplat_dropout": (_i, [
+        C.c_longlong, _i, _p, C.c_longlong, _p, C.c_longlong, C.c_double, C.c_ulonglong,
+        C.c_ulonglong, _i, _p,
+    ]),
+    "msplat_mx4_record_bytes": (_i, [_i]),
+    "msplat_mx4_pack": (_i, [_i, _i, _p, _p, _p, _p]),
+    "msplat_mx4_unpack": (_i, [_i, _i, _p, _p, _p, _p]),
+    "msplat_mx4_colors": (_i, [_i, _i, _i, _p, _p, _i, _p, _p, _p, _p]),
+    "msplat_mx4_colors_backward": (_i, [_i, _i, _i, _p, _i, _p, _p, _p, _p, _p, _p]),
     "msplat_last_loss": (_f, [_i]),
     "msplat_num_intersections": (C.c_longlong, []),
     "msplat_device_errors": (_i, []),

@@ -154,6 +154,17 @@ int engine_init() { return init_engine(); }
 cudaStream_t engine_stream() { return g.stream(); }
 const SideStream& engine_side() { return g.side; }
 void engine_add_launches(int n) { g.launches += n; }
+int launched(const char* who, int n)
+{
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) {
+        set_error("%s: %s", who, cudaGetErrorString(e));
+        return MSPLAT_ERR_CUDA;
+    }
+    std::lock_guard<std::mutex> lk(g_mu);
+    g.launches += n;
+    return MSPLAT_OK;
+}
 
 template <typename T>
 static int realloc_dev(T*& p, size_t count)

@@ -207,6 +207,7 @@ struct SideStream {
 };
 const SideStream& engine_side();        // stream all engine work goes to
 void engine_add_launches(int n);     // for msplat_kernel_launches
+int launched(const char* who, int n);  // status after n launches of a call outside the lock; counts them
 void stage_release();                // frees msplat_stage_input's buffers (engine lock held)
 
 // Host helpers shared by the entry points (engine.cu).

@@ -1,0 +1,161 @@
+"""Dropout and 4-bit colour operators, what needs no GPU: the plain
+implementations that the GPU tests hold the kernels to, and every refusal of
+the C-ABI and of msplat_b200.operators (checked before any CUDA call)."""
+from __future__ import annotations
+
+import ctypes as C
+import os
+
+import numpy as np
+import pytest
+import torch
+
+from msplat_b200 import _lib, build, operators
+from tests import operators_case as oc
+
+P = 0x1000  # an aligned address that a refused call must never read
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not os.path.exists(_lib.LIB_PATH):
+        build.build()
+    return _lib.load()
+
+
+# ---- the plain implementations
+
+@pytest.mark.parametrize("counter, key, want", [
+    ((0, 0), 0, (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+    ((2**64 - 1, 2**64 - 1), 2**64 - 1, (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+    ((0x85A308D3243F6A88, 0x0370734413198A2E), 0x299F31D0A4093822,
+     (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1)),
+])
+def test_philox_known_answers(counter, key, want):
+    got = oc.philox(np.array([counter[0]], np.uint64), counter[1], key)[0]
+    assert tuple(int(v) for v in got) == want
+
+
+def test_draws_are_uniform():
+    d = oc.draws(np.arange(40_000), step=7, seed=11)
+    # 6 standard deviations of a share of 40,000 draws
+    for t in (0.1, 0.5, 0.9):
+        assert abs((d < t * 2**32).mean() - t) < 6 * np.sqrt(t * (1 - t) / d.size)
+
+
+@pytest.mark.parametrize("degree", range(5))
+def test_record_values_are_nearest(degree):
+    dc, rest = oc.features(500, degree, seed=degree)
+    rdc, rrest = oc.decode(oc.encode(dc, rest), degree)
+    assert (np.abs(rdc - dc) <= 2.0**-11 * np.abs(dc) + 2.0**-25).all()
+    if degree:
+        # half the widest step of the grid is 2^e, and the largest at least 3.5 2^e
+        top = np.abs(rest).max(1, keepdims=True)
+        assert (np.abs(rrest - rest) <= top / 3.5).all()
+        # what a record stands for packs to itself
+        again = oc.encode(rdc.astype(np.float32), rrest.astype(np.float32))
+        np.testing.assert_array_equal(again, oc.encode(dc, rest))
+
+
+def test_record_bytes(lib):
+    assert [lib.msplat_mx4_record_bytes(d) for d in range(5)] == list(oc.BYTES)
+    assert tuple(operators.RECORD_BYTES) == oc.BYTES and tuple(operators.REST_BASES) == oc.REST
+
+
+# ---- refusals of the C-ABI
+
+def refused(lib, rc, *words):
+    assert rc == -1, rc
+    text = lib.msplat_last_error().decode()
+    for w in words:
+        assert w in text, text
+
+
+@pytest.mark.parametrize("change, words", [
+    (dict(rows=-1), ("invalid shape",)), (dict(cols=0), ("invalid shape",)),
+    (dict(xs=3), ("invalid shape",)), (dict(ys=3), ("invalid shape",)),
+    (dict(rows=2**61, cols=1, xs=0, ys=0), ("invalid shape",)),
+    (dict(rate=-0.1), ("rate",)), (dict(rate=1.0), ("rate",)), (dict(rate=float("nan")), ("rate",)),
+    (dict(rate=1 - 2.0**-40), ("rate",)),
+    (dict(x=None), ("null",)), (dict(y=None), ("null",)), (dict(y=P, xs=4, ys=5), ("in place",)),
+])
+def test_dropout_refusals(lib, change, words):
+    a = dict(rows=8, cols=4, x=P, xs=4, y=2 * P, ys=4, rate=0.5)
+    a.update(change)
+    rc = lib.msplat_dropout(a["rows"], a["cols"], a["x"], a["xs"], a["y"], a["ys"], a["rate"], 1, 2,
+                            0, None)
+    refused(lib, rc, "msplat_dropout", *words)
+
+
+@pytest.mark.parametrize("n, degree, dc, rest, rec, words", [
+    (-1, 3, P, P, P, ("invalid shape",)), (1, -1, P, P, P, ("invalid shape",)),
+    (1, 5, P, P, P, ("invalid shape",)), (1, 3, None, P, P, ("null",)), (1, 3, P, None, P, ("null",)),
+    (1, 3, P, P, None, ("aligned",)), (1, 3, P, P, P + 8, ("16-byte aligned",)),
+    (1, 2, P, P, P + 4, ("8-byte aligned",)),
+])
+def test_pack_refusals(lib, n, degree, dc, rest, rec, words):
+    refused(lib, lib.msplat_mx4_pack(n, degree, dc, rest, rec, None), "msplat_mx4_pack", *words)
+    refused(lib, lib.msplat_mx4_unpack(n, degree, rec, dc, rest, None), "msplat_mx4_unpack", *words)
+
+
+@pytest.mark.parametrize("change, words", [
+    (dict(n=-1), ("invalid shape",)), (dict(degree=5), ("invalid shape",)),
+    (dict(use=4), ("invalid arguments",)), (dict(use=-1), ("invalid arguments",)),
+    (dict(views=65), ("up to 64",)), (dict(views=-1), ("invalid arguments",)),
+    (dict(cams=None), ("invalid arguments",)), (dict(means=None), ("null",)), (dict(col=None), ("null",)),
+])
+def test_colors_refusals(lib, change, words):
+    a = dict(n=4, degree=3, use=3, means=P, rec=P, views=2, col=P, dc=P, rest=P,
+             cams=np.zeros(200, np.float32).ctypes.data)
+    a.update(change)
+    refused(lib, lib.msplat_mx4_colors(a["n"], a["degree"], a["use"], a["means"], a["rec"], a["views"],
+                                       a["cams"], None, a["col"], None), "msplat_mx4_colors", *words)
+    refused(lib, lib.msplat_mx4_colors_backward(a["n"], a["degree"], a["use"], a["means"], a["views"],
+                                                a["cams"], None, a["col"], a["dc"], a["rest"], None),
+            "msplat_mx4_colors_backward", *words)
+
+
+def test_colors_refuses_records(lib):
+    cams = np.zeros(3, np.float32).ctypes.data
+    for rec in (None, P + 8):
+        refused(lib, lib.msplat_mx4_colors(1, 3, 3, P, rec, 1, cams, None, P, None), "aligned")
+    for out in ((None, P), (P, None)):
+        refused(lib, lib.msplat_mx4_colors_backward(1, 3, 3, P, 1, cams, None, P, *out, None), "null")
+
+
+def test_nothing_to_do_is_no_error(lib):
+    """Empty calls succeed without a GPU: nothing is launched."""
+    assert lib.msplat_dropout(0, 1, None, 0, None, 0, 0.5, 1, 2, 0, None) == 0
+    assert lib.msplat_mx4_pack(0, 3, None, None, None, None) == 0
+    assert lib.msplat_mx4_unpack(0, 3, None, None, None, None) == 0
+    assert lib.msplat_mx4_colors(0, 3, 3, None, None, 0, None, None, None, None) == 0
+    assert lib.msplat_mx4_colors(5, 3, 3, None, None, 0, None, None, None, None) == 0
+    assert lib.msplat_mx4_colors_backward(0, 3, 3, None, 0, None, None, None, None, None, None) == 0
+
+
+# ---- refusals of the Python calls (a CPU tensor is one)
+
+def test_python_refusals():
+    x = torch.zeros(4, 3)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        operators.dropout(x, 0.5, 1, 2)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        operators.mx4_pack(x, torch.zeros(4, 15, 3))
+    with pytest.raises(ValueError, match="bases"):
+        operators.mx4_pack(x, torch.zeros(4, 14, 3))
+    with pytest.raises(ValueError, match=r"\(N, B, 3\)"):
+        operators.mx4_pack(x, x)
+    with pytest.raises(ValueError, match="degree"):
+        operators.mx4_unpack(torch.zeros(4, 32, dtype=torch.uint8), 7)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        operators.mx4_unpack(torch.zeros(4, 32, dtype=torch.uint8), 3)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        operators.mx4_colors(torch.zeros(4, 32, dtype=torch.uint8), 3, x, [[0, 0, 0]])
+    with pytest.raises(ValueError, match="degree"):
+        operators.mx4_colors_backward(torch.zeros(1, 4, 3), 5, x, [[0, 0, 0]])
+    with pytest.raises(ValueError, match="degrees_to_use"):
+        operators.mx4_colors_backward(torch.zeros(1, 4, 3), 2, x, [[0, 0, 0]], degrees_to_use=3)
+    with pytest.raises(ValueError, match="V <= 64"):
+        operators.mx4_colors_backward(torch.zeros(65, 4, 3), 2, x, np.zeros((65, 3)))
+    with pytest.raises(ValueError, match="host data"):
+        operators.mx4_colors_backward(torch.zeros(1, 4, 3), 2, x, torch.zeros(1, 3))
