@@ -162,6 +162,11 @@ public:
     Trainer(const Trainer&) = delete;
     Trainer& operator=(const Trainer&) = delete;
 
+    // Training options beyond the reference's configuration (MsplatTrainerOptions).
+    void setOptions(const MsplatTrainerOptions& options)
+    {
+        if (msplat_trainer_set_options(t_, &options) != 0) detail::fail("msplat::Trainer::setOptions");
+    }
     Stats step()
     {
         const MsplatStats s = msplat_trainer_step(t_);

@@ -105,6 +105,21 @@ void msplat_dataset_camera_pose(MsplatDataset ds, int cameraIndex, float camToWo
 MsplatTrainer msplat_trainer_create(MsplatDataset ds, MsplatConfig config);
 void msplat_trainer_destroy(MsplatTrainer t);
 
+/* Options of the training steps beyond the reference's configuration; all
+ * zeros (the reference's training) until set.
+ *   dropoutRate, dropoutSeed  dropout of whole Gaussians in every step (the
+ *     iteration counts the steps, so a resumed run draws as an uninterrupted
+ *     one); 0 <= dropoutRate < 1
+ *   mx4Colors  train with 4-bit colours, and render and evaluate with them
+ * See MsplatStepOptions in msplat_engine.h.  0, or -1 with msplat_last_error
+ * set (the earlier options then stay). */
+typedef struct {
+    double dropoutRate;
+    unsigned long long dropoutSeed;
+    bool mx4Colors;
+} MsplatTrainerOptions;
+int msplat_trainer_set_options(MsplatTrainer t, const MsplatTrainerOptions *options);
+
 MsplatStats msplat_trainer_step(MsplatTrainer t);
 /* Steps until config.iterations. */
 void msplat_trainer_train(MsplatTrainer t);

@@ -128,6 +128,31 @@ int msplat_train_step(
     float *max_2d_size, float inv_max_dim, const int32_t **radii_out, float *loss_out);
 
 /*
+ * Options of the training steps; no counterpart in the reference.  They hold
+ * for every later msplat_train_step, _grads, _grads_compact and
+ * _grads_accumulate of this process, until set again; NULL, and the state at
+ * the start, is all zeros: the reference's step.  Renders are not affected.
+ *   dropout_rate  dropout of whole Gaussians, the regulariser for scenes with
+ *     few views (0 <= rate < 1; 0: none).  A Gaussian whose draw (msplat_dropout
+ *     with whole rows: key dropout_seed, counter (Gaussian, dropout_step))
+ *     drops it takes no part in the step, as if the view culled it; the
+ *     opacity of the others is multiplied by 1 / (1 - rate), in the gradient
+ *     too.  Set dropout_step anew for each step.  The views of one step, and
+ *     ranks, that are given the same seed and step drop the same Gaussians.
+ *   mx4_colors  the forward pass takes its colours from 4-bit records of the
+ *     features (see msplat_mx4_pack); gradients go straight through the
+ *     rounding to the float features.  What is trained then is what
+ *     msplat_render_mx4 shows.  Needs degree <= 4 and features_rest_bases =
+ *     (degree + 1)^2 - 1.
+ */
+typedef struct MsplatStepOptions {
+    double dropout_rate;
+    unsigned long long dropout_seed, dropout_step;
+    int mx4_colors;
+} MsplatStepOptions;
+int msplat_set_step_options(const MsplatStepOptions *options);
+
+/*
  * Data-parallel training, gradient half.  No counterpart in the reference
  * (which trains one view on one device); it is msplat_train_step with the
  * fused optimiser replaced by a gradient output, so that ranks training
@@ -256,6 +281,19 @@ int msplat_render(
     float clip_thresh, unsigned degree, unsigned degrees_to_use, const float *cam_pos,
     const float *features_dc, const float *features_rest, const float *opacities,
     const float *background, float **out_img);
+
+/*
+ * Forward-only render of a scene whose colours are 4-bit records
+ * (msplat_mx4_pack with SH degree `degree`, 0 to 4): msplat_render with
+ * `records` for features_dc and features_rest, and the image that it would
+ * give for the unpacked features, bit for bit.
+ */
+int msplat_render_mx4(
+    int num_points, const float *means3d, const float *scales, float glob_scale,
+    const float *quats, const float *viewmat, const float *projmat, float fx, float fy,
+    float cx, float cy, unsigned img_height, unsigned img_width, const int *tile_bounds,
+    float clip_thresh, unsigned degree, unsigned degrees_to_use, const float *cam_pos,
+    const void *records, const float *opacities, const float *background, float **out_img);
 
 /*
  * Forward-only render that allocates nothing.  No counterpart in the

@@ -42,6 +42,17 @@ class MsplatConfig(C.Structure):
     ]
 
 
+class MsplatStepOptions(C.Structure):
+    """MsplatStepOptions (include/msplat_engine.h)."""
+    _fields_ = [("dropout_rate", C.c_double), ("dropout_seed", C.c_ulonglong),
+                ("dropout_step", C.c_ulonglong), ("mx4_colors", C.c_int)]
+
+
+class MsplatTrainerOptions(C.Structure):
+    """MsplatTrainerOptions (include/msplat_c_api.h)."""
+    _fields_ = [("dropoutRate", C.c_double), ("dropoutSeed", C.c_ulonglong), ("mx4Colors", C.c_bool)]
+
+
 class MsplatStats(C.Structure):
     _fields_ = [("iteration", C.c_int), ("splatCount", C.c_int), ("msPerStep", C.c_float)]
 
@@ -179,6 +190,12 @@ SIGNATURES = {
         _i, _p, _p, _f, _p, _fp, _fp, _f, _f, _f, _f, _u, _u, _ip, _f, _u, _u, _fp,
         _p, _p, _p, _fp, _p, _p,
     ]),
+    "msplat_set_step_options": (_i, [C.POINTER(MsplatStepOptions)]),
+    "msplat_render_mx4": (_i, [
+        _i, _p, _p, _f, _p, _fp, _fp, _f, _f, _f, _f, _u, _u, _ip, _f, _u, _u, _fp,
+        _p, _p, _fp, C.POINTER(_p),
+    ]),
+    "msplat_trainer_set_options": (_i, [_p, C.POINTER(MsplatTrainerOptions)]),
     "msplat_dropout": (_i, [
         C.c_longlong, _i, _p, C.c_longlong, _p, C.c_longlong, C.c_double, C.c_ulonglong,
         C.c_ulonglong, _i, _p,

@@ -39,8 +39,11 @@ struct StepParams {
     int num_adam_groups;
     int prefix_sort;  // tiles of more than kSortRun keys sort their nearest keys only
     int dense_bins;   // binning for views of many tiles per Gaussian (kDenseArea)
-    int pad0;
+    unsigned drop_threshold;  // dropout of Gaussians (training with a rate above 0 only)
     long long capacity;
+    unsigned long long drop_seed, drop_step;
+    float drop_scale;         // factor of the kept ones' opacity
+    float drop_inv;           // 1 / drop_scale
 };
 
 // Dense binning (StepParams::dense_bins, set by the host when the last view
@@ -105,6 +108,7 @@ struct Buffers {
     int* chunk_idx;        // [K*H*W]
     float* prefix_T;       // [K*H*W]
     float* after_C;        // [K*H*W*3]
+    void* records;         // training with 4-bit colours only: this step's records
     float* loss_sum;       // [1]
     int* err;              // [1]
     int* isect_total;      // [1] intersections of the view (scan output), or null
@@ -207,6 +211,16 @@ struct SideStream {
 };
 const SideStream& engine_side();        // stream all engine work goes to
 void engine_add_launches(int n);     // for msplat_kernel_launches
+// Options of the training steps (msplat_set_step_options), checked.
+struct StepOptions {
+    bool dropout = false, mx4 = false;
+    unsigned threshold = 0;
+    float scale = 1.f;
+    unsigned long long seed = 0, step = 0;
+};
+bool make_step_options(const char* who, double rate, unsigned long long seed,
+                       unsigned long long step, bool mx4, StepOptions* out);
+StepOptions swap_step_options(const StepOptions& o);  // sets them; returns the earlier ones
 int launched(const char* who, int n);  // status after n launches of a call outside the lock; counts them
 void stage_release();                // frees msplat_stage_input's buffers (engine lock held)
 
@@ -219,7 +233,14 @@ int chunk_k_max(long long N, int num_tiles);           // depth chunks of one ti
 void launch_project_forward(const StepParams* P, int N, const float* means, const float* scales,
                             const float* quats, const float* dc, const float* rest,
                             const float* opac, const Buffers& B, bool zero_grads,
-                            int degrees_to_use_host, int rest_stride_host, cudaStream_t s);
+                            int degrees_to_use_host, int rest_stride_host, cudaStream_t s,
+                            bool colors = true, bool dropout = false);
+// 4-bit colours (kernels_mx4.cu), for callers that checked the arguments.
+void launch_mx4_pack(int n, int degree, const float* dc, const float* rest, void* records,
+                     cudaStream_t s);
+void launch_mx4_rgb(int n, int degree, int use, const float* means, const void* records,
+                    const float* cam_pos, const int* radii, float4* rgb, cudaStream_t s);
+bool mx4_records_ok(const char* who, const void* records, int degree);
 void launch_scan_tiles(const StepParams* P, int num_tiles, bool dense_bins, const Buffers& B,
                        cudaStream_t s);
 void launch_scatter(const StepParams* P, int N, const Buffers& B, cudaStream_t s);
@@ -233,7 +254,7 @@ void launch_raster_forward(const StepParams* P, int num_tiles, int k_max, bool p
 void launch_ssim(const StepParams* P, int W, int H, const float* gt, const Buffers& B,
                  cudaStream_t s);
 void launch_raster_backward(const StepParams* P, int num_tiles, int k_max, int W, int H,
-                            const Buffers& B, cudaStream_t s);
+                            const Buffers& B, bool dropout, cudaStream_t s);
 // Returns the number of kernels launched (the SH-rest Adam runs as its own kernel).
 int launch_project_backward_adam(const StepParams* P, int N, int degrees_to_use_host,
                                  int rest_stride_host, const Buffers& B, const AdamPtrs& A,

@@ -104,7 +104,9 @@ __device__ __forceinline__ bool backprop(PixelBwd& s, float fpx, float fpy, cons
     return true;
 }
 
-template <bool CHUNKED, int PPT>
+// DROPOUT: co.w is the sigmoid s times drop_scale, and the derivative with
+// respect to the logit needs 1 - s.
+template <bool CHUNKED, int PPT, bool DROPOUT>
 __global__ void __launch_bounds__(256 / PPT, kBwdMinBlocks)
 raster_backward_kernel(const StepParams* __restrict__ P, const int* __restrict__ offset,
                        const int* __restrict__ order, const int* __restrict__ ids,
@@ -305,7 +307,7 @@ raster_backward_kernel(const StepParams* __restrict__ P, const int* __restrict__
                     if (j >= 3 && j < 6) x *= 0.5f;
                     if (ok) atomicAdd(grad_acc + (size_t)g * kGradStride + j, x);
                 } else if (lane == 1) {
-                    if (vop != 0.f) atomicAdd(grad_acc + (size_t)g * kGradStride + 8, -(1.f - co.w) * vop);
+                    if (vop != 0.f) atomicAdd(grad_acc + (size_t)g * kGradStride + 8, -(1.f - (DROPOUT ? co.w * P->drop_inv : co.w)) * vop);
                 }
             }
         }
@@ -351,21 +353,30 @@ chunk_prefix_suffix_kernel(const StepParams* __restrict__ P, const int* __restri
 }
 
 void launch_raster_backward(const StepParams* P, int num_tiles, int k_max, int W, int H,
-                            const Buffers& B, cudaStream_t s)
+                            const Buffers& B, bool dropout, cudaStream_t s)
 {
     if (num_tiles <= 0) return;
     if (k_max <= 1) {
-        raster_backward_kernel<false, kBwdPPT><<<num_tiles, 256 / kBwdPPT, 0, s>>>(
-            P, B.tile_offset, B.tile_order, B.sorted_ids, B.proj.xy, B.proj.conic_op, B.proj.rgb, B.final_T,
-            B.final_idx, B.v_rendered, nullptr, nullptr, nullptr, nullptr, B.grad_acc);
+        auto run = [&](auto kernel) {
+            kernel<<<num_tiles, 256 / kBwdPPT, 0, s>>>(
+                P, B.tile_offset, B.tile_order, B.sorted_ids, B.proj.xy, B.proj.conic_op, B.proj.rgb,
+                B.final_T, B.final_idx, B.v_rendered, nullptr, nullptr, nullptr, nullptr, B.grad_acc);
+        };
+        dropout ? run(raster_backward_kernel<false, kBwdPPT, true>)
+                : run(raster_backward_kernel<false, kBwdPPT, false>);
     } else {
         dim3 pgrid((W + 15) / 16, (H + 15) / 16);
         chunk_prefix_suffix_kernel<<<pgrid, 256, 0, s>>>(P, B.tile_offset, B.chunk_T, B.chunk_C,
                                                          B.prefix_T, B.after_C);
         dim3 grid(num_tiles, k_max);
-        raster_backward_kernel<true, kBwdPPT><<<grid, 256 / kBwdPPT, 0, s>>>(
-            P, B.tile_offset, B.tile_order, B.sorted_ids, B.proj.xy, B.proj.conic_op, B.proj.rgb, B.final_T,
-            nullptr, B.v_rendered, B.chunk_idx, B.prefix_T, B.chunk_T, B.after_C, B.grad_acc);
+        auto run = [&](auto kernel) {
+            kernel<<<grid, 256 / kBwdPPT, 0, s>>>(
+                P, B.tile_offset, B.tile_order, B.sorted_ids, B.proj.xy, B.proj.conic_op, B.proj.rgb,
+                B.final_T, nullptr, B.v_rendered, B.chunk_idx, B.prefix_T, B.chunk_T, B.after_C,
+                B.grad_acc);
+        };
+        dropout ? run(raster_backward_kernel<true, kBwdPPT, true>)
+                : run(raster_backward_kernel<true, kBwdPPT, false>);
     }
 }
 

@@ -2,6 +2,7 @@
 // per-tile depth sort and the forward rasterizer.  Compiled with
 // --fmad=false (see msp_math.cuh): every value here is bit-identical to the
 // CPU oracle.
+#include "dropout.cuh"
 #include "engine.h"
 #include "msp_math.cuh"
 #include "tma.cuh"
@@ -96,7 +97,12 @@ struct ProjStage {
 // block is full and the arrays are 16-byte aligned, else by plain loads.
 // Every byte of the block is then in flight at once instead of in two
 // dependent rounds (geometry, then the SH rows of the visible Gaussians).
-template <bool ZERO_GRADS>
+// Without COLORS the colours come from 4-bit records: dc and rest are
+// neither staged nor read, and out.rgb is left to another kernel.  With
+// DROPOUT a Gaussian that its draw drops is culled -- not binned, sorted,
+// blended nor given gradients -- and the others' opacity is multiplied by
+// drop_scale.
+template <bool ZERO_GRADS, bool COLORS, bool DROPOUT>
 __global__ void __launch_bounds__(kProjThreads)
 project_forward_kernel(const StepParams* __restrict__ P, int N, const float* __restrict__ means,
                        const float* __restrict__ scales, const float* __restrict__ quats,
@@ -124,13 +130,13 @@ project_forward_kernel(const StepParams* __restrict__ P, int N, const float* __r
         if (tid == 0) mbar_init(&s_bar);
         __syncthreads();
         if (tid == 0) {
-            const unsigned rs_bytes = (unsigned)(kProjThreads * rest_stride * 4);
-            mbar_expect_tx(&s_bar, (unsigned)(ProjStage::kRest * 4) + rs_bytes);
+            const unsigned rs_bytes = COLORS ? (unsigned)(kProjThreads * rest_stride * 4) : 0u;
+            mbar_expect_tx(&s_bar, (unsigned)((COLORS ? ProjStage::kRest : ProjStage::kDc) * 4) + rs_bytes);
             bulk_load(sm + ProjStage::kMeans, means + gb * 3, kProjThreads * 12, &s_bar);
             bulk_load(sm + ProjStage::kScales, scales + gb * 3, kProjThreads * 12, &s_bar);
             bulk_load(sm + ProjStage::kQuats, quats + gb * 4, kProjThreads * 16, &s_bar);
             bulk_load(sm + ProjStage::kOpac, opac + gb, kProjThreads * 4, &s_bar);
-            bulk_load(sm + ProjStage::kDc, dc + gb * 3, kProjThreads * 12, &s_bar);
+            if (COLORS) bulk_load(sm + ProjStage::kDc, dc + gb * 3, kProjThreads * 12, &s_bar);
             if (rs_bytes) bulk_load(sm + ProjStage::kRest, rest + gb * rest_stride, rs_bytes, &s_bar);
             s_fail = !mbar_wait_bounded(&s_bar, 0);
             if (s_fail) {
@@ -147,12 +153,13 @@ project_forward_kernel(const StepParams* __restrict__ P, int N, const float* __r
         for (int e = tid; e < cnt * 3; e += kProjThreads) {
             sm[ProjStage::kMeans + e] = means[gb * 3 + e];
             sm[ProjStage::kScales + e] = scales[gb * 3 + e];
-            sm[ProjStage::kDc + e] = dc[gb * 3 + e];
+            if (COLORS) sm[ProjStage::kDc + e] = dc[gb * 3 + e];
         }
         for (int e = tid; e < cnt * 4; e += kProjThreads) sm[ProjStage::kQuats + e] = quats[gb * 4 + e];
         if (tid < cnt) sm[ProjStage::kOpac + tid] = opac[gb + tid];
-        for (int e = tid; e < cnt * rest_stride; e += kProjThreads)
-            sm[ProjStage::kRest + e] = rest[gb * rest_stride + e];
+        if (COLORS)
+            for (int e = tid; e < cnt * rest_stride; e += kProjThreads)
+                sm[ProjStage::kRest + e] = rest[gb * rest_stride + e];
         __syncthreads();
     }
 
@@ -252,12 +259,15 @@ project_forward_kernel(const StepParams* __restrict__ P, int N, const float* __r
                 y0 = min(max(0, f2i(tcy - try_)), P->tiles_y);
                 y1 = min(max(0, f2i((tcy + try_) + 1)), P->tiles_y);
                 int area = (x1 - x0) * (y1 - y0);
-                if (area > 0) {
+                if (area > 0 && (!DROPOUT || dropout_draw((unsigned)i, P->drop_step, P->drop_seed) >=
+                                                 P->drop_threshold)) {
                     vis = true;
                     out.radii[i] = f2i(radius);
                     out.depth[i] = pv2;
                     out.xy[i] = make_float2(px_c, py_c);
-                    out.conic_op[i] = make_float4(ca, cb, cc, sigmoid_ref(s_opac[tid]));
+                    float op = sigmoid_ref(s_opac[tid]);
+                    if (DROPOUT) op *= P->drop_scale;
+                    out.conic_op[i] = make_float4(ca, cb, cc, op);
                     out.rect[i] = make_uint2((unsigned)x0 | ((unsigned)y0 << 16),
                                              (unsigned)x1 | ((unsigned)y1 << 16));
                 }
@@ -265,13 +275,15 @@ project_forward_kernel(const StepParams* __restrict__ P, int N, const float* __r
         }
     }
     if (!vis) return;
-    // SH colour (:1780-1786): viewdir = normalize(p - cam_pos)
-    float d0 = p[0] - P->cam_pos[0], d1 = p[1] - P->cam_pos[1], d2 = p[2] - P->cam_pos[2];
-    float dn = rsqrt_ieee((d0 * d0 + d1 * d1) + d2 * d2);
-    float col[3];
-    float dcv[3] = {s_dc[3 * tid], s_dc[3 * tid + 1], s_dc[3 * tid + 2]};
-    sh_to_color(P->degrees_to_use, d0 * dn, d1 * dn, d2 * dn, dcv, s_rest + tid * rest_stride, col);
-    out.rgb[i] = make_float4(col[0], col[1], col[2], 0.f);
+    if constexpr (COLORS) {
+        // SH colour (:1780-1786): viewdir = normalize(p - cam_pos)
+        float d0 = p[0] - P->cam_pos[0], d1 = p[1] - P->cam_pos[1], d2 = p[2] - P->cam_pos[2];
+        float dn = rsqrt_ieee((d0 * d0 + d1 * d1) + d2 * d2);
+        float col[3];
+        float dcv[3] = {s_dc[3 * tid], s_dc[3 * tid + 1], s_dc[3 * tid + 2]};
+        sh_to_color(P->degrees_to_use, d0 * dn, d1 * dn, d2 * dn, dcv, s_rest + tid * rest_stride, col);
+        out.rgb[i] = make_float4(col[0], col[1], col[2], 0.f);
+    }
     if (ZERO_GRADS) {  // training: the SH-rest Adam's copy of the mean
         out.sh_mean[3 * (size_t)i] = p[0];
         out.sh_mean[3 * (size_t)i + 1] = p[1];
@@ -300,23 +312,31 @@ project_forward_kernel(const StepParams* __restrict__ P, int N, const float* __r
 void launch_project_forward(const StepParams* P, int N, const float* means, const float* scales,
                             const float* quats, const float* dc, const float* rest,
                             const float* opac, const Buffers& B, bool zero_grads,
-                            int degrees_to_use_host, int rest_stride_host, cudaStream_t s)
+                            int degrees_to_use_host, int rest_stride_host, cudaStream_t s,
+                            bool colors, bool dropout)
 {
     (void)degrees_to_use_host;
     if (N <= 0) return;
-    const size_t smem = (size_t)(ProjStage::kRest + kProjThreads * rest_stride_host) * sizeof(float);
-    const uintptr_t mis = (uintptr_t)means | (uintptr_t)scales | (uintptr_t)quats |
-                          (uintptr_t)dc | (uintptr_t)opac | (rest_stride_host ? (uintptr_t)rest : 0);
+    const size_t smem = (size_t)(colors ? ProjStage::kRest + kProjThreads * rest_stride_host
+                                        : ProjStage::kDc) * sizeof(float);
+    uintptr_t mis = (uintptr_t)means | (uintptr_t)scales | (uintptr_t)quats | (uintptr_t)opac;
+    if (colors) mis |= (uintptr_t)dc | (rest_stride_host ? (uintptr_t)rest : 0);
     const int bulk = (mis & 15) == 0 && smem <= 48 * 1024;
     const int grid = (N + kProjThreads - 1) / kProjThreads;
-    if (zero_grads)
-        project_forward_kernel<true><<<grid, kProjThreads, smem, s>>>(
-            P, N, means, scales, quats, dc, rest, opac, B.proj, B.tile_count, B.grad_acc,
-            rest_stride_host, bulk, B.err);
+    auto run = [&](auto kernel) {
+        kernel<<<grid, kProjThreads, smem, s>>>(P, N, means, scales, quats, dc, rest, opac, B.proj,
+                                                B.tile_count, zero_grads ? B.grad_acc : nullptr,
+                                                rest_stride_host, bulk, B.err);
+    };
+    if (!zero_grads)  // a render: nothing is dropped
+        colors ? run(project_forward_kernel<false, true, false>)
+               : run(project_forward_kernel<false, false, false>);
+    else if (!dropout)
+        colors ? run(project_forward_kernel<true, true, false>)
+               : run(project_forward_kernel<true, false, false>);
     else
-        project_forward_kernel<false><<<grid, kProjThreads, smem, s>>>(
-            P, N, means, scales, quats, dc, rest, opac, B.proj, B.tile_count, nullptr,
-            rest_stride_host, bulk, B.err);
+        colors ? run(project_forward_kernel<true, true, true>)
+               : run(project_forward_kernel<true, false, true>);
 }
 
 // ---------------------------------------------------------------------------

@@ -136,6 +136,31 @@ mx4_colors_kernel(int n, int use, const float* __restrict__ means,
     }
 }
 
+// One view's colours of the visible Gaussians, into the renderer's buffer.
+template <int DEG>
+__global__ void __launch_bounds__(kMxThreads)
+mx4_rgb_kernel(int n, int use, const float* __restrict__ means,
+               const void* __restrict__ records, float3 cam, const int* __restrict__ radii,
+               float4* __restrict__ rgb)
+{
+    const long long i = (long long)blockIdx.x * kMxThreads + threadIdx.x;
+    if (i >= n || radii[i] <= 0) return;
+    const float cp[3] = {cam.x, cam.y, cam.z};
+    float p[3], d[3], dc[3], s[3] = {0.f, 0.f, 0.f}, col[3];
+#pragma unroll
+    for (int k = 0; k < 3; k++) p[k] = means[3 * i + k];
+    unsigned w[mx4_words(DEG)];
+    mx4_load<DEG>(records, i, w);
+    mx4_dc(w, dc);
+    if constexpr (DEG > 0) mx4_scales(w, s);
+    view_dir(cp, p, d);
+    const ShDir D = sh_dir(d);
+#pragma unroll
+    for (int c = 0; c < 3; c++)
+        col[c] = mx4_color<DEG>(use, D, dc[c], s[c], [&](int k) { return mx4_code(w, 3 * k + c); });
+    rgb[i] = make_float4(col[0], col[1], col[2], 0.f);
+}
+
 template <int DEG>
 __global__ void __launch_bounds__(kMxThreads)
 mx4_colors_backward_kernel(int n, int use, const float* __restrict__ means, int views,
@@ -215,14 +240,6 @@ bool check_shape(const char* who, int n, int degree)
     return true;
 }
 
-bool check_records(const char* who, const void* records, int degree)
-{
-    if (records && ((uintptr_t)records & (mx4_align(degree) - 1)) == 0) return true;
-    set_error("%s: records of degree %d must be a %d-byte aligned device pointer", who, degree,
-              mx4_align(degree));
-    return false;
-}
-
 bool check_views(const char* who, int degree, int degrees_to_use, int views, const float* cam_pos,
                  Mx4Cams* cams)
 {
@@ -244,6 +261,35 @@ int null_pointer(const char* who)
 }
 
 }  // namespace
+
+bool mx4_records_ok(const char* who, const void* records, int degree)
+{
+    if (records && ((uintptr_t)records & (mx4_align(degree) - 1)) == 0) return true;
+    set_error("%s: records of degree %d must be a %d-byte aligned device pointer", who, degree,
+              mx4_align(degree));
+    return false;
+}
+
+void launch_mx4_pack(int n, int degree, const float* dc, const float* rest, void* records,
+                     cudaStream_t s)
+{
+    if (n <= 0) return;
+    with_degree(degree, [&](auto D) {
+        mx4_pack_kernel<D.value><<<blocks_for(n), kMxThreads, 0, s>>>(n, dc, rest, records);
+    });
+}
+
+void launch_mx4_rgb(int n, int degree, int use, const float* means, const void* records,
+                    const float* cam_pos, const int* radii, float4* rgb, cudaStream_t s)
+{
+    if (n <= 0) return;
+    const float3 cam = make_float3(cam_pos[0], cam_pos[1], cam_pos[2]);
+    with_degree(degree, [&](auto D) {
+        mx4_rgb_kernel<D.value><<<blocks_for(n), kMxThreads, 0, s>>>(n, use, means, records, cam,
+                                                                     radii, rgb);
+    });
+}
+
 }  // namespace msp
 
 using namespace msp;
@@ -263,12 +309,9 @@ int msplat_mx4_pack(int n, int degree, const float* features_dc, const float* fe
     if (!check_shape(who, n, degree)) return MSPLAT_ERR_ARG;
     if (n == 0) return MSPLAT_OK;
     if (!features_dc || (degree > 0 && !features_rest)) return null_pointer(who);
-    if (!check_records(who, records, degree)) return MSPLAT_ERR_ARG;
-    const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
-    with_degree(degree, [&](auto D) {
-        mx4_pack_kernel<D.value><<<blocks_for(n), kMxThreads, 0, st>>>(n, features_dc,
-                                                                        features_rest, records);
-    });
+    if (!mx4_records_ok(who, records, degree)) return MSPLAT_ERR_ARG;
+    launch_mx4_pack(n, degree, features_dc, features_rest, records,
+                    static_cast<cudaStream_t>(cuda_stream));
     return launched(who, 1);
 }
 
@@ -279,7 +322,7 @@ int msplat_mx4_unpack(int n, int degree, const void* records, float* features_dc
     if (!check_shape(who, n, degree)) return MSPLAT_ERR_ARG;
     if (n == 0) return MSPLAT_OK;
     if (!features_dc || (degree > 0 && !features_rest)) return null_pointer(who);
-    if (!check_records(who, records, degree)) return MSPLAT_ERR_ARG;
+    if (!mx4_records_ok(who, records, degree)) return MSPLAT_ERR_ARG;
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     with_degree(degree, [&](auto D) {
         mx4_unpack_kernel<D.value><<<blocks_for(n), kMxThreads, 0, st>>>(n, records, features_dc,
@@ -299,7 +342,7 @@ int msplat_mx4_colors(int n, int degree, int degrees_to_use, const float* means3
         return MSPLAT_ERR_ARG;
     if (n == 0 || num_views == 0) return MSPLAT_OK;
     if (!means3d || !colors) return null_pointer(who);
-    if (!check_records(who, records, degree)) return MSPLAT_ERR_ARG;
+    if (!mx4_records_ok(who, records, degree)) return MSPLAT_ERR_ARG;
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     with_degree(degree, [&](auto D) {
         mx4_colors_kernel<D.value><<<blocks_for(n), kMxThreads, 0, st>>>(

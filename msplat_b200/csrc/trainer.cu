@@ -103,6 +103,9 @@ struct Model {
     float* v[kGroupsC] = {};
     float* stats[3] = {};  // vis_counts, xys_grad_norm, max_2d_size
     float* samples = nullptr;
+    bool mx4 = false;         // render from 4-bit records of the colours
+    void* records = nullptr;  // of the latest render
+    size_t records_bytes = 0;
     bool radii_defined = false;
     int lastHeight = 0, lastWidth = 0;
 
@@ -129,6 +132,8 @@ struct Model {
         for (auto& s : stats)
             if (s) cudaFree(s), s = nullptr;
         if (samples) cudaFree(samples), samples = nullptr;
+        if (records) cudaFree(records), records = nullptr;
+        records_bytes = 0;
         capacity = 0;
     }
 
@@ -314,10 +319,33 @@ struct Model {
         const CamSetup s = prepare_cam(cam, step);
         *w = s.width;
         *h = s.height;
+        if (mx4) return render_mx4(s, out);
         return msplat_render(num_active, buf[0], buf[1], 1.0f, buf[2], s.viewmat, s.projmat, s.fx,
                              s.fy, s.cx, s.cy, (unsigned)s.height, (unsigned)s.width, s.tiles,
                              0.01f, (unsigned)s.degree, (unsigned)s.degrees_to_use, s.cam_pos,
                              buf[3], buf[4], buf[5], bg, out);
+    }
+
+    int render_mx4(const CamSetup& s, float** out)
+    {
+        const size_t bytes = (size_t)num_active * msplat_mx4_record_bytes(s.degree);
+        if (bytes > records_bytes) {
+            if (records) cudaFree(records);
+            records = nullptr;
+            records_bytes = 0;
+            if (cudaMalloc(&records, bytes) != cudaSuccess) {
+                cudaGetLastError();
+                set_error("out of device memory for the records of %d Gaussians", num_active);
+                return MSPLAT_ERR_CUDA;
+            }
+            records_bytes = bytes;
+        }
+        const int rc = msplat_mx4_pack(num_active, s.degree, buf[3], buf[4], records, engine_stream());
+        if (rc) return rc;
+        return msplat_render_mx4(num_active, buf[0], buf[1], 1.0f, buf[2], s.viewmat, s.projmat,
+                                 s.fx, s.fy, s.cx, s.cy, (unsigned)s.height, (unsigned)s.width,
+                                 s.tiles, 0.01f, (unsigned)s.degree, (unsigned)s.degrees_to_use,
+                                 s.cam_pos, records, buf[5], bg, out);
     }
 
     // Model::fullIteration
@@ -438,6 +466,7 @@ struct TTrainer {
     std::vector<size_t> order;
     size_t pos = 0;
     std::mt19937 rng{42};
+    MsplatTrainerOptions opts{};
 
     void shuffle()
     {
@@ -456,6 +485,13 @@ struct TTrainer {
         *dataset_index = list[index];
         return msplat_dataset_camera(ds->data, list[index], info) == MSPLAT_OK;
     }
+};
+
+// The trainer's own step options for the length of one step.
+struct StepOptionsScope {
+    StepOptions before;
+    explicit StepOptionsScope(const StepOptions& o) : before(swap_step_options(o)) {}
+    ~StepOptionsScope() { swap_step_options(before); }
 };
 
 MsplatPixelBuffer download_rgb(const float* dev, int w, int h)
@@ -551,6 +587,22 @@ void msplat_trainer_destroy(MsplatTrainer t)
     delete static_cast<TTrainer*>(t);
 }
 
+int msplat_trainer_set_options(MsplatTrainer tp, const MsplatTrainerOptions* options)
+{
+    static const char* const who = "msplat_trainer_set_options";
+    auto* t = static_cast<TTrainer*>(tp);
+    if (!t || !options) {
+        set_error("%s: no trainer or no options", who);
+        return MSPLAT_ERR_ARG;
+    }
+    StepOptions checked;
+    if (!make_step_options(who, options->dropoutRate, 0, 0, options->mx4Colors, &checked))
+        return MSPLAT_ERR_ARG;
+    t->opts = *options;
+    t->model.mx4 = options->mx4Colors;
+    return MSPLAT_OK;
+}
+
 MsplatStats msplat_trainer_step(MsplatTrainer tp)
 {
     MsplatStats st{0, 0, 0.f};
@@ -568,8 +620,15 @@ MsplatStats msplat_trainer_step(MsplatTrainer tp)
     const float* gt = nullptr;
     int gw = 0, gh = 0;
     if (msplat_dataset_gt(t->ds->data, dsi, factor, &gt, &gw, &gh) != MSPLAT_OK) return st;
+    StepOptions opt;
+    if (!make_step_options("msplat_trainer_step", t->opts.dropoutRate, t->opts.dropoutSeed,
+                           (unsigned long long)t->current, t->opts.mx4Colors, &opt))
+        return st;
     const auto t0 = std::chrono::high_resolution_clock::now();
-    if (t->model.full_iteration(cam, t->current, gt, t->cfg.ssimWeight) != MSPLAT_OK) return st;
+    {
+        const StepOptionsScope scope(opt);
+        if (t->model.full_iteration(cam, t->current, gt, t->cfg.ssimWeight) != MSPLAT_OK) return st;
+    }
     t->model.schedulers_step(t->current);
     if (t->model.after_train(t->current) != MSPLAT_OK) return st;
     msplat_commit();

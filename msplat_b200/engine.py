@@ -320,6 +320,56 @@ def _ptr_array(ts):
     return (C.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
 
 
+def set_step_options(dropout_rate: float = 0.0, dropout_seed: int = 0, dropout_step: int = 0,
+                     mx4_colors: bool = False) -> None:
+    """msplat_set_step_options: dropout of whole Gaussians and 4-bit colours
+    in every later training step (train_step and the data-parallel halves);
+    without arguments, the reference's step again."""
+    m64 = 2**64 - 1
+    o = _lib.MsplatStepOptions(float(dropout_rate), int(dropout_seed) & m64, int(dropout_step) & m64,
+                               int(bool(mx4_colors)))
+    if _lib.load().msplat_set_step_options(C.byref(o)) != 0:
+        raise ValueError(_lib.load().msplat_last_error().decode())
+
+
+class PackedGaussians:
+    """A scene to render whose SH coefficients are 4-bit records
+    (operators.mx4_pack): 76 bytes per Gaussian at SH degree 3 instead of
+    236.  means, scales, quats and opacities are those of a GaussianModel."""
+
+    def __init__(self, means, scales, quats, opacities, records, sh_degree: int):
+        self.means, self.scales, self.quats, self.opacities = means, scales, quats, opacities
+        self.records, self.sh_degree = records, int(sh_degree)
+
+    @classmethod
+    def of(cls, model: GaussianModel) -> "PackedGaussians":
+        """The model's Gaussians as they are now: copies, on torch's current
+        stream (bind_stream() makes it the engine's)."""
+        from . import operators
+        p = model.params
+        return cls(p[0].clone(), p[1].clone(), p[2].clone(), p[5].clone(),
+                   operators.mx4_pack(p[3], p[4]), model.sh_degree)
+
+    @property
+    def n(self) -> int:
+        return int(self.means.shape[0])
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in
+                   (self.means, self.scales, self.quats, self.opacities, self.records))
+
+    def features(self):
+        """(features_dc, features_rest) that the records stand for."""
+        from . import operators
+        return operators.mx4_unpack(self.records, self.sh_degree)
+
+    def colors(self, cam_pos, degrees_to_use=None):
+        """Raw SH colours (V, N, 3) from camera positions (V, 3; host)."""
+        from . import operators
+        return operators.mx4_colors(self.records, self.sh_degree, self.means, cam_pos, degrees_to_use)
+
+
 def train_step(model: GaussianModel, cam: CamSetup, gt, ssim_weight: float = 0.2,
                background=DEFAULT_BG, glob_scale: float = 1.0, clip_thresh: float = 0.01):
     """One msplat_train_step; returns the engine's loss value (see
@@ -360,6 +410,21 @@ def render(model: GaussianModel, cam: CamSetup, background=DEFAULT_BG, glob_scal
         cam.degrees_to_use, _lib.farr(cam.cam_pos), _ptr(p[3]), _ptr(p[4]), _ptr(p[5]),
         _lib.farr(background), C.byref(out))
     _lib.check(rc, "msplat_render")
+    return int(out.value)
+
+
+def render_mx4(packed: PackedGaussians, cam: CamSetup, background=DEFAULT_BG,
+               glob_scale: float = 1.0, clip_thresh: float = 0.01) -> int:
+    """msplat_render_mx4; returns the device address of the (H,W,3) image."""
+    lib = _lib.load()
+    out = C.c_void_p()
+    rc = lib.msplat_render_mx4(
+        packed.n, _ptr(packed.means), _ptr(packed.scales), glob_scale, _ptr(packed.quats),
+        _lib.farr(cam.viewmat), _lib.farr(cam.projmat), cam.fx, cam.fy, cam.cx, cam.cy,
+        cam.height, cam.width, _lib.iarr(cam.tile_bounds), clip_thresh, packed.sh_degree,
+        min(cam.degrees_to_use, packed.sh_degree), _lib.farr(cam.cam_pos), _ptr(packed.records),
+        _ptr(packed.opacities), _lib.farr(background), C.byref(out))
+    _lib.check(rc, "msplat_render_mx4")
     return int(out.value)
 
 

@@ -113,6 +113,17 @@ class GaussianTrainer:
         except Exception:  # noqa: BLE001 -- interpreter shutdown
             pass
 
+    def set_options(self, dropout_rate: float = 0.0, dropout_seed: int = 0,
+                    mx4_colors: bool = False) -> None:
+        """Training options beyond the reference's configuration
+        (MsplatTrainerOptions in include/msplat_c_api.h): dropout of whole
+        Gaussians in every step, and 4-bit colours in training, rendering
+        and evaluation.  They replace the earlier ones."""
+        o = _lib.MsplatTrainerOptions(float(dropout_rate), int(dropout_seed) & (2**64 - 1),
+                                      bool(mx4_colors))
+        if _lib.load().msplat_trainer_set_options(self._t, C.byref(o)) != 0:
+            raise ValueError(_lib.load().msplat_last_error().decode())
+
     def step(self) -> TrainingStats:
         s = _lib.load().msplat_trainer_step(self._t)
         if s.iteration == 0:

@@ -159,3 +159,24 @@ def test_python_refusals():
         operators.mx4_colors_backward(torch.zeros(65, 4, 3), 2, x, np.zeros((65, 3)))
     with pytest.raises(ValueError, match="host data"):
         operators.mx4_colors_backward(torch.zeros(1, 4, 3), 2, x, torch.zeros(1, 3))
+
+
+# ---- options of the training step and the packed renderer
+
+def test_option_refusals(lib):
+    for rate in (-0.5, 1.0, float("nan")):
+        refused(lib, lib.msplat_set_step_options(C.byref(_lib.MsplatStepOptions(rate, 1, 2, 0))),
+                "msplat_set_step_options", "rate")
+    assert lib.msplat_set_step_options(C.byref(_lib.MsplatStepOptions(0.5, 1, 2, 1))) == 0
+    assert lib.msplat_set_step_options(None) == 0
+    refused(lib, lib.msplat_trainer_set_options(None, C.byref(_lib.MsplatTrainerOptions())), "no trainer")
+
+
+@pytest.mark.parametrize("degree, rec, words", [(5, P, ("degree 5",)), (3, None, ("aligned",)),
+                                                (3, P + 8, ("16-byte aligned",))])
+def test_render_mx4_refusals(lib, degree, rec, words):
+    m = (C.c_float * 16)()
+    out = C.c_void_p()
+    rc = lib.msplat_render_mx4(4, P, P, 1.0, P, m, m, 1.0, 1.0, 0.0, 0.0, 16, 16, (C.c_int * 3)(1, 1, 1),
+                               0.01, degree, min(degree, 3), m, rec, P, m, C.byref(out))
+    refused(lib, rc, "msplat_render_mx4", *words)
