@@ -1,8 +1,9 @@
 // kernels_dropout.cu -- dropout of an array's rows or elements
 // (msplat_dropout).  y = x * scale where kept, 0 where dropped; its backward
 // pass is the same map on the gradient, under the same seed and step.
-// A pass reads and writes four bytes per element, and one Philox block
-// (about 60 integer operations) serves four draws.
+// A pass reads and writes four bytes per element, and one Philox block (ten
+// rounds of two wide multiplications and two three-way exclusive ors) serves
+// four draws.
 #include <algorithm>
 
 #include "dropout.cuh"
@@ -20,71 +21,201 @@ struct DropArgs {
     int cols;
     unsigned threshold;
     float scale;
-    unsigned long long seed, step;
+    unsigned long long step;
+    PhiloxKeys keys;
 };
 
-// One draw per element.  A thread takes the four elements of one Philox
-// group, which lie side by side in the array when it has no gaps (FLAT);
-// VEC: 16-byte accesses.
-template <bool FLAT, bool VEC>
+// One draw per element, arrays without gaps at 16-byte alignment.  A thread
+// takes the four elements of one Philox group as one vector.  40M elements:
+// 54 us (5.9 TB/s).
 __global__ void __launch_bounds__(kDropThreads)
-dropout_elements_kernel(DropArgs a, long long total)
+dropout_vector_kernel(DropArgs a, long long total)
 {
     const long long groups = (total + 3) >> 2;
     for (long long g = blockIdx.x * (long long)kDropThreads + threadIdx.x; g < groups;
          g += (long long)gridDim.x * kDropThreads) {
         const long long i0 = g << 2;
-        const uint4 d = philox4x32((unsigned long long)g, a.step, a.seed);
-        const unsigned u[4] = {d.x, d.y, d.z, d.w};
-        if (VEC && i0 + 4 <= total) {
-            float4 v = *reinterpret_cast<const float4*>(a.x + i0);
-            v.x = u[0] >= a.threshold ? v.x * a.scale : 0.f;
-            v.y = u[1] >= a.threshold ? v.y * a.scale : 0.f;
-            v.z = u[2] >= a.threshold ? v.z * a.scale : 0.f;
-            v.w = u[3] >= a.threshold ? v.w * a.scale : 0.f;
+        const bool whole = i0 + 4 <= total;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (whole) v = *reinterpret_cast<const float4*>(a.x + i0);   // in flight under the draws
+        const uint4 d = philox4x32((unsigned long long)g, a.step, a.keys);
+        if (whole) {
+            v.x = d.x >= a.threshold ? v.x * a.scale : 0.f;
+            v.y = d.y >= a.threshold ? v.y * a.scale : 0.f;
+            v.z = d.z >= a.threshold ? v.z * a.scale : 0.f;
+            v.w = d.w >= a.threshold ? v.w * a.scale : 0.f;
             *reinterpret_cast<float4*>(a.y + i0) = v;
-            continue;
-        }
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const long long i = i0 + k;
-            if (i >= total) break;
-            long long ix = i, iy = i;
-            if (!FLAT) {
-                const long long r = i / a.cols, c = i - r * a.cols;
-                ix = r * a.x_stride + c;
-                iy = r * a.y_stride + c;
-            }
-            a.y[iy] = u[k] >= a.threshold ? a.x[ix] * a.scale : 0.f;
+        } else {
+            const unsigned u[4] = {d.x, d.y, d.z, d.w};
+            for (int k = 0; i0 + k < total; k++)
+                a.y[i0 + k] = u[k] >= a.threshold ? a.x[i0 + k] * a.scale : 0.f;
         }
     }
 }
 
-// One draw per row.  A block draws for kDropRows rows, then streams them.
-constexpr int kDropRows = 128;
-__global__ void __launch_bounds__(kDropThreads)
-dropout_rows_kernel(DropArgs a)
+// The other kernels give a block a chunk of consecutive elements: one 64-bit
+// division finds the chunk's first row, and an element's row and column in
+// the chunk come from 32-bit arithmetic.  (Dividing each element's 64-bit
+// index took 34 us a pass over 333,337 rows of 23, of which the traffic is 10.)
+constexpr int kChunkElems = 8192;
+
+// Row of place t = (column of the chunk's first element) + (element of the
+// chunk), counted from the chunk's first row.  Exact: t < cols + 8192 and, by
+// `magic` = ceil(2^32 / cols) for 2 <= cols <= 8192, t * cols < 2^32.
+enum RowRule { kOneColumn, kByMagic, kWideRows };
+template <RowRule RULE>
+__device__ __forceinline__ int local_row(unsigned t, int cols, unsigned magic)
 {
-    __shared__ float s_scale[kDropRows];
-    const long long chunks = (a.rows + kDropRows - 1) / kDropRows;
+    return RULE == kByMagic ? (int)__umulhi(t, magic)
+         : RULE == kOneColumn ? (int)t : (int)(t >= (unsigned)cols);
+}
+
+// One draw per element, any strides and alignment.  A warp takes 256
+// elements; each lane draws two groups' four, and ballots turn the draws into
+// a bit per element, so that every access is of 32 neighbours and not of each
+// lane's own four.  Offset: the type that holds a row offset in a chunk (32
+// bits for all but the widest strides).  Bound by instructions, the draws'
+// and the indexes': 333,337 rows of 23 in rows of 27, 16.5 us a pass (3.7
+// TB/s); 40M elements off alignment 83 us.  48 registers (5 blocks a
+// multiprocessor) 18.1 us, 78 without that bound 21.4.  `magic64` = ceil(2^64 / cols) divides the chunk's first
+// index exactly while index * cols < 2^64; 0: plain division.
+constexpr int kElemsChunk = 256 * (kDropThreads / 32);
+
+template <RowRule RULE, typename Offset, bool FULL>
+__device__ __forceinline__ void dropout_chunk(const DropArgs& a, long long i0, int cnt,
+                                              unsigned magic, unsigned long long magic64)
+{
+    const int lane = threadIdx.x & 31;
+    const int e0 = 256 * (threadIdx.x >> 5) + lane;
+    const long long r0 = magic64 ? (long long)__umul64hi((unsigned long long)i0, magic64) : i0 / a.cols;
+    const unsigned c0 = (unsigned)(i0 - r0 * a.cols);
+    const float* x = a.x + r0 * a.x_stride;
+    float* y = a.y + r0 * a.y_stride;
+    float v[8];
+    Offset to[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const unsigned t = c0 + e0 + 32 * k;
+        const int r = local_row<RULE>(t, a.cols, magic);
+        const int c = (int)(t - (unsigned)r * (unsigned)a.cols);
+        to[k] = (Offset)r * (Offset)a.y_stride + c;
+        v[k] = 0.f;
+        if (FULL || e0 + 32 * k < cnt) v[k] = x[(Offset)r * (Offset)a.x_stride + c];   // in flight under the draws
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const uint4 d = philox4x32((unsigned long long)((i0 + e0 - lane) >> 2) + 32 * h + lane,
+                                   a.step, a.keys);
+        const unsigned b0 = __ballot_sync(0xffffffffu, d.x >= a.threshold);
+        const unsigned b1 = __ballot_sync(0xffffffffu, d.y >= a.threshold);
+        const unsigned b2 = __ballot_sync(0xffffffffu, d.z >= a.threshold);
+        const unsigned b3 = __ballot_sync(0xffffffffu, d.w >= a.threshold);
+        // element 32 k + lane: word lane & 3 of group 8 k + lane / 4
+        const unsigned word = (lane & 2 ? (lane & 1 ? b3 : b2) : (lane & 1 ? b1 : b0)) >> (lane >> 2);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (FULL || e0 + 128 * h + 32 * k < cnt)
+                y[to[4 * h + k]] = (word >> (8 * k)) & 1u ? v[4 * h + k] * a.scale : 0.f;
+    }
+}
+
+template <RowRule RULE, typename Offset>
+__global__ void __launch_bounds__(kDropThreads, 5)
+dropout_elements_kernel(DropArgs a, long long total, unsigned magic, unsigned long long magic64)
+{
+    const long long chunks = (total + kElemsChunk - 1) / kElemsChunk;
     for (long long ch = blockIdx.x; ch < chunks; ch += gridDim.x) {
-        const long long r0 = ch * kDropRows;
-        const int cnt = (int)min((long long)kDropRows, a.rows - r0);
+        const long long i0 = ch * kElemsChunk;
+        if (i0 + kElemsChunk <= total)
+            dropout_chunk<RULE, Offset, true>(a, i0, kElemsChunk, magic, magic64);
+        else
+            dropout_chunk<RULE, Offset, false>(a, i0, (int)(total - i0), magic, magic64);
+    }
+}
+
+// One draw per row: a block draws for its chunk's rows into shared memory,
+// then streams the elements; dropped ones are not read.
+// VEC: rows side by side, 16-byte alignment -- four elements an access, of at
+// most two rows (with two columns too: a chunk starts at a row then, so an
+// access starts at one).  1M rows of 45 at rate 0.2, both directions: 106 us
+// (6.8 TB/s of the bytes of all rows; the dropped fifth is not read), against
+// 292 with an element an access.
+template <RowRule RULE, bool VEC>
+__global__ void __launch_bounds__(kDropThreads)
+dropout_rows_kernel(DropArgs a, long long total, unsigned magic)
+{
+    __shared__ float s_scale[kChunkElems / 2 + 8];   // the rows of a chunk: at least 2 columns
+    const long long chunks = (total + kChunkElems - 1) / kChunkElems;
+    for (long long ch = blockIdx.x; ch < chunks; ch += gridDim.x) {
+        const long long i0 = ch * kChunkElems;
+        const long long r0 = i0 / a.cols;
+        const unsigned c0 = (unsigned)(i0 - r0 * a.cols);
+        const int cnt = (int)min((long long)kChunkElems, total - i0);
+        const long long g0 = r0 >> 2;
+        const int skip = (int)(r0 & 3);   // s_scale starts at the row of the first group
+        const int rows = skip + local_row<RULE>(c0 + cnt - 1, a.cols, magic) + 1;
         __syncthreads();
-        if (threadIdx.x < kDropRows / 4) {
-            const uint4 d = philox4x32((unsigned long long)(r0 >> 2) + threadIdx.x, a.step, a.seed);
-            s_scale[4 * threadIdx.x] = d.x >= a.threshold ? a.scale : 0.f;
-            s_scale[4 * threadIdx.x + 1] = d.y >= a.threshold ? a.scale : 0.f;
-            s_scale[4 * threadIdx.x + 2] = d.z >= a.threshold ? a.scale : 0.f;
-            s_scale[4 * threadIdx.x + 3] = d.w >= a.threshold ? a.scale : 0.f;
+        for (int g = threadIdx.x; 4 * g < rows; g += kDropThreads) {
+            const uint4 d = philox4x32((unsigned long long)(g0 + g), a.step, a.keys);
+            s_scale[4 * g] = d.x >= a.threshold ? a.scale : 0.f;
+            s_scale[4 * g + 1] = d.y >= a.threshold ? a.scale : 0.f;
+            s_scale[4 * g + 2] = d.z >= a.threshold ? a.scale : 0.f;
+            s_scale[4 * g + 3] = d.w >= a.threshold ? a.scale : 0.f;
         }
         __syncthreads();
-        const long long total = (long long)cnt * a.cols;
-        for (long long e = threadIdx.x; e < total; e += kDropThreads) {
-            const int r = (int)(e / a.cols);
-            const int c = (int)(e - (long long)r * a.cols);
-            const float f = s_scale[r];   // a dropped value may be anything, a NaN too: no product
-            a.y[(r0 + r) * a.y_stride + c] = f != 0.f ? a.x[(r0 + r) * a.x_stride + c] * f : 0.f;
+        const float* scale = s_scale + skip;
+        if (VEC) {
+            const float* x = a.x + i0;
+            float* y = a.y + i0;
+            const int vecs = cnt >> 2;
+            constexpr int kU = 4;
+            for (int b = threadIdx.x; b < vecs; b += kDropThreads * kU) {
+                float4 v[kU];
+                float f0[kU], f1[kU];
+                int edge[kU];
+#pragma unroll
+                for (int u = 0; u < kU; u++) {
+                    const int q = b + u * kDropThreads;
+                    if (q >= vecs) continue;
+                    const unsigned t = c0 + 4u * q;
+                    const int r = local_row<RULE>(t, a.cols, magic);
+                    edge[u] = (int)((unsigned)(r + 1) * (unsigned)a.cols - t);   // elements left of row r
+                    f0[u] = scale[r];
+                    f1[u] = edge[u] < 4 ? scale[r + 1] : f0[u];
+                    v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (f0[u] != 0.f || f1[u] != 0.f) v[u] = reinterpret_cast<const float4*>(x)[q];
+                }
+#pragma unroll
+                for (int u = 0; u < kU; u++) {
+                    const int q = b + u * kDropThreads;
+                    if (q >= vecs) continue;
+                    const float g1 = edge[u] > 1 ? f0[u] : f1[u], g2 = edge[u] > 2 ? f0[u] : f1[u],
+                                g3 = edge[u] > 3 ? f0[u] : f1[u];
+                    // a dropped value may be anything, a NaN too: no product
+                    v[u].x = f0[u] != 0.f ? v[u].x * f0[u] : 0.f;
+                    v[u].y = g1 != 0.f ? v[u].y * g1 : 0.f;
+                    v[u].z = g2 != 0.f ? v[u].z * g2 : 0.f;
+                    v[u].w = g3 != 0.f ? v[u].w * g3 : 0.f;
+                    reinterpret_cast<float4*>(y)[q] = v[u];
+                }
+            }
+            const int e = 4 * vecs + threadIdx.x;
+            if (e < cnt) {
+                const float f = scale[local_row<RULE>(c0 + e, a.cols, magic)];
+                y[e] = f != 0.f ? x[e] * f : 0.f;
+            }
+            continue;
+        }
+        const float* x = a.x + r0 * a.x_stride;
+        float* y = a.y + r0 * a.y_stride;
+#pragma unroll 4
+        for (int e = threadIdx.x; e < cnt; e += kDropThreads) {
+            const unsigned t = c0 + e;
+            const int r = local_row<RULE>(t, a.cols, magic);
+            const int c = (int)(t - (unsigned)r * (unsigned)a.cols);
+            const float f = scale[r];
+            const float v = f != 0.f ? x[r * a.x_stride + c] : 0.f;
+            y[r * a.y_stride + c] = v * f;
         }
     }
 }
@@ -117,20 +248,47 @@ extern "C" int msplat_dropout(long long rows, int cols, const float* x, long lon
                                                  : "in place needs the same row stride twice");
         return MSPLAT_ERR_ARG;
     }
-    const DropArgs a{x, y, rows, x_stride, y_stride, cols, dr.threshold, dr.scale, seed, step};
+    const DropArgs a{x, y, rows, x_stride, y_stride, cols, dr.threshold, dr.scale, step, philox_keys(seed)};
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+    const long long total = rows * cols;
+    const bool flat = x_stride == cols && y_stride == cols;
+    const bool aligned = flat && (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
+    auto blocks = [](long long items, long long per) {
+        return (unsigned)std::min<long long>((items + per - 1) / per, 1 << 20);
+    };
+    const unsigned magic =
+        cols >= 2 && cols <= kChunkElems ? (unsigned)(((1ULL << 32) + cols - 1) / cols) : 0u;
     if (whole_rows && cols > 1) {
-        const long long chunks = (rows + kDropRows - 1) / kDropRows;
-        dropout_rows_kernel<<<(unsigned)std::min<long long>(chunks, 1 << 20), kDropThreads, 0, st>>>(a);
+        auto run = [&](auto kernel) {
+            kernel<<<blocks(total, kChunkElems), kDropThreads, 0, st>>>(a, total, magic);
+        };
+        if (aligned)
+            magic ? run(dropout_rows_kernel<kByMagic, true>) : run(dropout_rows_kernel<kWideRows, true>);
+        else
+            magic ? run(dropout_rows_kernel<kByMagic, false>) : run(dropout_rows_kernel<kWideRows, false>);
+    } else if (aligned) {
+        dropout_vector_kernel<<<blocks(total, 4 * kDropThreads), kDropThreads, 0, st>>>(a, total);
     } else {
-        const long long total = rows * cols;
-        const bool flat = x_stride == cols && y_stride == cols;
-        const bool vec = flat && (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
-        const unsigned blocks = (unsigned)std::min<long long>(
-            ((total + 3) / 4 + kDropThreads - 1) / kDropThreads, 1 << 20);
-        if (vec) dropout_elements_kernel<true, true><<<blocks, kDropThreads, 0, st>>>(a, total);
-        else if (flat) dropout_elements_kernel<true, false><<<blocks, kDropThreads, 0, st>>>(a, total);
-        else dropout_elements_kernel<false, false><<<blocks, kDropThreads, 0, st>>>(a, total);
+        DropArgs e = a;
+        if (flat) {  // one long row: an element's index is its place
+            e.cols = 1 << 29;
+            e.x_stride = e.y_stride = e.cols;
+        }
+        const bool fits = e.cols > 1 && total < (1LL << 62) / e.cols;
+        const unsigned long long magic64 = fits ? ~0ULL / (unsigned)e.cols + 1 : 0;
+        const bool narrow = (kElemsChunk / e.cols + 2) * std::max(e.x_stride, e.y_stride) < 1LL << 31;
+        auto run = [&](auto kernel) {
+            kernel<<<blocks(total, kElemsChunk), kDropThreads, 0, st>>>(e, total, magic, magic64);
+        };
+        if (e.cols == 1)
+            narrow ? run(dropout_elements_kernel<kOneColumn, int>)
+                   : run(dropout_elements_kernel<kOneColumn, long long>);
+        else if (e.cols <= kChunkElems)
+            narrow ? run(dropout_elements_kernel<kByMagic, int>)
+                   : run(dropout_elements_kernel<kByMagic, long long>);
+        else
+            narrow ? run(dropout_elements_kernel<kWideRows, int>)
+                   : run(dropout_elements_kernel<kWideRows, long long>);
     }
     return launched("msplat_dropout", 1);
 }
