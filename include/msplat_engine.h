@@ -615,8 +615,8 @@ int msplat_mx4_unpack(int n, int degree, const void *records, float *features_dc
  * (num_views,3; host): colors (num_views,n,3) = the SH basis of the direction
  * from the camera to the mean, times the coefficients; degrees up to
  * degrees_to_use (<= degree).  The raw colour, as the rasterizer takes it
- * (it adds 0.5 and clamps at 0).  Bit for bit what the renderer computes from the
- * unpacked coefficients.  With radii (num_views,n; NULL: all visible) the
+ * (it adds 0.5 and clamps at 0); the sums are fused multiply-adds, so its last
+ * bits are not the renderer's.  With radii (num_views,n; NULL: all visible) the
  * colours of Gaussians of radius <= 0 are not written.  A mean at the camera
  * has no direction: its colour is NaN unless degrees_to_use is 0. */
 int msplat_mx4_colors(int n, int degree, int degrees_to_use, const float *means3d,

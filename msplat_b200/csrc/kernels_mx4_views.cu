@@ -1,0 +1,259 @@
+// kernels_mx4_views.cu -- the colours of a batch of views from 4-bit records
+// (format in mx4.cuh) and the gradient of the coefficients.  Compiled with FMA
+// contraction: a fused multiply-add per coefficient and view is what bounds
+// many views.  (A renderer's view, kernels_mx4.cu, keeps the projection's bits.)
+#include "mx4_rows.cuh"
+
+namespace msp {
+namespace {
+
+// Unit direction from a camera to a mean: the hardware's reciprocal square
+// root (2^-22.9) and one Newton step.  IEEE root and division, as the
+// projection has them, are a third of a view's instructions.
+__device__ __forceinline__ void unit_dir(const float* cam, const float p[3], float d[3])
+{
+    const float d0 = p[0] - cam[0], d1 = p[1] - cam[1], d2 = p[2] - cam[2];
+    const float n = fmaf(d2, d2, fmaf(d1, d1, d0 * d0));
+    float r;
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(n));
+    r = fmaf(0.5f * r, fmaf(-(n * r), r, 1.f), r);
+    d[0] = d0 * r;
+    d[1] = d1 * r;
+    d[2] = d2 * r;
+}
+
+// SH basis values beside dc of degrees 1 to DEG (sh_to_color's convention).
+template <int DEG>
+__device__ __forceinline__ void sh_basis(const float d[3], float* b)
+{
+    if constexpr (DEG == 0) return;
+    const float x = d[0], y = d[1], z = d[2];
+    b[0] = -MSP_SH_C1 * y;
+    b[1] = MSP_SH_C1 * z;
+    b[2] = -MSP_SH_C1 * x;
+    if constexpr (DEG >= 2) {
+        const float xx = x * x, yy = y * y, zz = z * z, xy = x * y, yz = y * z, xz = x * z;
+        const float xmy = xx - yy;
+        b[3] = kSH_C2[0] * xy;
+        b[4] = kSH_C2[1] * yz;
+        b[5] = kSH_C2[2] * (fmaf(2.f, zz, -xx) - yy);
+        b[6] = kSH_C2[3] * xz;
+        b[7] = kSH_C2[4] * xmy;
+        if constexpr (DEG >= 3) {
+            const float u = fmaf(3.f, xx, -yy), v = fmaf(-3.f, yy, xx), w = fmaf(4.f, zz, -xx) - yy;
+            b[8] = kSH_C3[0] * y * u;
+            b[9] = kSH_C3[1] * xy * z;
+            b[10] = kSH_C3[2] * y * w;
+            b[11] = kSH_C3[3] * z * fmaf(2.f, zz, -3.f * (xx + yy));
+            b[12] = kSH_C3[4] * x * w;
+            b[13] = kSH_C3[5] * z * xmy;
+            b[14] = kSH_C3[6] * x * v;
+            if constexpr (DEG >= 4) {
+                const float s = fmaf(7.f, zz, -1.f), t = fmaf(7.f, zz, -3.f);
+                b[15] = kSH_C4[0] * xy * xmy;
+                b[16] = kSH_C4[1] * yz * u;
+                b[17] = kSH_C4[2] * xy * s;
+                b[18] = kSH_C4[3] * yz * t;
+                b[19] = kSH_C4[4] * fmaf(zz, fmaf(35.f, zz, -30.f), 3.f);
+                b[20] = kSH_C4[5] * xz * t;
+                b[21] = kSH_C4[6] * xmy * s;
+                b[22] = kSH_C4[7] * xz * v;
+                b[23] = kSH_C4[8] * fmaf(xx, v, -(yy * u));
+            }
+        }
+    }
+}
+
+// Views of `radii` that see Gaussian i, as bits; all of them without radii.
+__device__ __forceinline__ unsigned long long views_of(const int* radii, long long i, long long n,
+                                                       int views)
+{
+    if (!radii) return ~0ull >> (64 - views);
+    unsigned long long seen = 0;
+    for (int v = 0; v < views; v++)
+        if (radii[v * n + i] > 0) seen |= 1ull << v;
+    return seen;
+}
+
+// DEG: the records' degree; USE: the degrees in use.
+template <int DEG, int USE>
+__global__ void __launch_bounds__(kMxThreads)
+mx4_colors_kernel(int n, const float* __restrict__ means, const void* __restrict__ records,
+                  int views, const Mx4Cams cams, const int* __restrict__ radii,
+                  float* __restrict__ colors)
+{
+    constexpr int B = mx4_rest(USE);
+    __shared__ float s_col[kMxThreads * 3];
+    const int tid = threadIdx.x, lane = tid & 31, w0 = tid & ~31;
+    const long long base = (long long)blockIdx.x * kMxThreads;
+    const long long i = base + tid;
+    const unsigned long long seen = i < n ? views_of(radii, i, n, views) : 0ull;
+    float p[3] = {0.f, 0.f, 0.f}, dc[3] = {0.f, 0.f, 0.f}, s[3] = {0.f, 0.f, 0.f};
+    float q[3 * mx4_rest(DEG) + 1];
+    if (seen) {
+        unsigned w[mx4_words(DEG)];
+#pragma unroll
+        for (int k = 0; k < 3; k++) p[k] = means[3 * i + k];
+        mx4_load<DEG>(records, i, w);
+        mx4_dc(w, dc);
+#pragma unroll
+        for (int c = 0; c < 3; c++) dc[c] *= MSP_SH_C0;
+        if constexpr (USE > 0) {
+            mx4_scales(w, s);
+            mx4_codes<DEG>(w, q);
+        }
+    }
+    for (int v = 0; v < views; v++) {
+        const bool on = (seen >> v) & 1ull;
+        if (on) {
+            float col[3] = {dc[0], dc[1], dc[2]};
+            if constexpr (USE > 0) {
+                float d[3], b[B];
+                unit_dir(cams.p[v], p, d);
+                sh_basis<USE>(d, b);
+#pragma unroll
+                for (int c = 0; c < 3; c++) {
+                    float sum = b[0] * q[c];
+#pragma unroll
+                    for (int k = 1; k < B; k++) sum = fmaf(b[k], q[3 * k + c], sum);
+                    col[c] = fmaf(s[c], sum, dc[c]);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 3; c++) s_col[3 * tid + c] = col[c];
+        }
+        const unsigned bal = __ballot_sync(0xffffffffu, on);
+        __syncwarp();
+        float* out = colors + (v * (long long)n + base + w0) * 3;
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            const int e = 32 * k + lane;
+            if ((bal >> (e / 3)) & 1u) out[e] = s_col[3 * w0 + e];
+        }
+        __syncwarp();
+    }
+}
+
+template <int DEG, int USE>
+__global__ void __launch_bounds__(kMxThreads)
+mx4_colors_backward_kernel(int n, const float* __restrict__ means, int views, const Mx4Cams cams,
+                           const int* __restrict__ radii, const float* __restrict__ v_colors,
+                           float* __restrict__ v_dc, float* __restrict__ v_rest)
+{
+    constexpr int B = mx4_rest(USE), E = 3 * mx4_rest(DEG), PITCH = mx4_pitch<DEG>();
+    __shared__ float s_dc[kMxThreads * 3];
+    __shared__ float s_rest[E ? kMxThreads * PITCH : 1];
+    const long long base = (long long)blockIdx.x * kMxThreads;
+    const long long i = base + threadIdx.x;
+    const int cnt = (int)min((long long)kMxThreads, n - base);
+    if (i < n) {
+        const unsigned long long seen = views > 0 ? views_of(radii, i, n, views) : 0ull;
+        float gd[3] = {0.f, 0.f, 0.f}, gr[3 * B + 1];
+#pragma unroll
+        for (int e = 0; e < 3 * B; e++) gr[e] = 0.f;
+        float p[3];
+#pragma unroll
+        for (int k = 0; k < 3; k++) p[k] = means[3 * i + k];
+        for (int v = 0; v < views; v++) {
+            if (!((seen >> v) & 1ull)) continue;
+            float g[3];
+#pragma unroll
+            for (int c = 0; c < 3; c++) {
+                g[c] = v_colors[(v * (long long)n + i) * 3 + c];
+                gd[c] += g[c];
+            }
+            if constexpr (USE > 0) {
+                float d[3], b[B];
+                unit_dir(cams.p[v], p, d);
+                sh_basis<USE>(d, b);
+#pragma unroll
+                for (int k = 0; k < B; k++)
+#pragma unroll
+                    for (int c = 0; c < 3; c++) gr[3 * k + c] = fmaf(b[k], g[c], gr[3 * k + c]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 3; c++) s_dc[3 * threadIdx.x + c] = MSP_SH_C0 * gd[c];
+#pragma unroll
+        for (int e = 0; e < E; e++) s_rest[threadIdx.x * PITCH + e] = e < 3 * B ? gr[e < 3 * B ? e : 0] : 0.f;
+    }
+    __syncthreads();
+    rows_out<3, 3>(v_dc + base * 3, s_dc, cnt);
+    if constexpr (E > 0) rows_out<E, PITCH>(v_rest + base * E, s_rest, cnt);
+}
+
+bool views_ok(const char* who, int degree, int degrees_to_use, int views, const float* cam_pos,
+              Mx4Cams* cams)
+{
+    if (degrees_to_use < 0 || degrees_to_use > degree || views < 0 || views > kMx4MaxViews ||
+        (views > 0 && !cam_pos)) {
+        set_error("%s: invalid arguments (degree %d in use of %d, %d views; up to %d views)", who,
+                  degrees_to_use, degree, views, kMx4MaxViews);
+        return false;
+    }
+    for (int v = 0; v < views; v++)
+        for (int k = 0; k < 3; k++) cams->p[v][k] = cam_pos[3 * v + k];
+    return true;
+}
+
+// f(degree, degrees in use), both checked, as std::integral_constants.
+template <typename F>
+void with_degrees(int degree, int use, F f)
+{
+    with_degree(degree, [&](auto D) {
+        with_degree(use, [&](auto U) {
+            if constexpr (U.value <= D.value) f(D, U);
+        });
+    });
+}
+
+}  // namespace
+}  // namespace msp
+
+using namespace msp;
+
+extern "C" {
+
+int msplat_mx4_colors(int n, int degree, int degrees_to_use, const float* means3d,
+                      const void* records, int num_views, const float* cam_pos,
+                      const int32_t* radii, float* colors, void* cuda_stream)
+{
+    static const char* const who = "msplat_mx4_colors";
+    Mx4Cams cams;
+    if (!mx4_shape_ok(who, n, degree) ||
+        !views_ok(who, degree, degrees_to_use, num_views, cam_pos, &cams))
+        return MSPLAT_ERR_ARG;
+    if (n == 0 || num_views == 0) return MSPLAT_OK;
+    if (!means3d || !colors) return mx4_null_pointer(who);
+    if (!mx4_records_ok(who, records, degree)) return MSPLAT_ERR_ARG;
+    const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+    with_degrees(degree, degrees_to_use, [&](auto D, auto U) {
+        mx4_colors_kernel<D.value, U.value><<<mx4_blocks(n), kMxThreads, 0, st>>>(
+            n, means3d, records, num_views, cams, radii, colors);
+    });
+    return launched(who, 1);
+}
+
+int msplat_mx4_colors_backward(int n, int degree, int degrees_to_use, const float* means3d,
+                               int num_views, const float* cam_pos, const int32_t* radii,
+                               const float* v_colors, float* v_features_dc,
+                               float* v_features_rest, void* cuda_stream)
+{
+    static const char* const who = "msplat_mx4_colors_backward";
+    Mx4Cams cams;
+    if (!mx4_shape_ok(who, n, degree) ||
+        !views_ok(who, degree, degrees_to_use, num_views, cam_pos, &cams))
+        return MSPLAT_ERR_ARG;
+    if (n == 0) return MSPLAT_OK;
+    if (!means3d || (num_views > 0 && !v_colors) || !v_features_dc ||
+        (degree > 0 && !v_features_rest))
+        return mx4_null_pointer(who);
+    const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+    with_degrees(degree, degrees_to_use, [&](auto D, auto U) {
+        mx4_colors_backward_kernel<D.value, U.value><<<mx4_blocks(n), kMxThreads, 0, st>>>(
+            n, means3d, num_views, cams, radii, v_colors, v_features_dc, v_features_rest);
+    });
+    return launched(who, 1);
+}
+
+}  // extern "C"

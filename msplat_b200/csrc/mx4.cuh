@@ -115,15 +115,53 @@ __device__ __forceinline__ void mx4_encode(const float* dc, const float* row,
     }
 }
 
-// Element j's code as a float, unscaled.  The sign, exponent and mantissa
-// bits of e2m1 placed in a float's own fields give value * 2^-126 (a
-// subnormal for the codes 0 and 0.5, as in e2m1).
-template <int W>
-__device__ __forceinline__ float mx4_code(const unsigned (&w)[W], int j)
+// The codes of a record as floats, unscaled.  The conversion instruction takes
+// a byte, two codes; by shifts and masks a pair takes eight instructions of the
+// integer pipe and ran at less than half the rate.  The byte is masked out
+// first and narrowed from 32 bits: with the word unpacked into four byte
+// registers, or the byte narrowed from 16 bits, this compiler (12.9) reads the
+// wrong byte where some of a word's bytes are not used.
+__device__ __forceinline__ float2 e2m1x2_floats(unsigned byte)
 {
-    const int nib = j + 18;  // bytes 0-8 are 18 nibbles
-    const unsigned n = w[nib >> 3] >> ((nib & 7) * 4);
-    return __uint_as_float((n & 8u) << 28 | (n & 7u) << 22) * 0x1p126f;
+    unsigned h;
+    asm("{\n\t"
+        ".reg .b8 a;\n\t"
+        "cvt.u8.u32 a, %1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+        "}"
+        : "=r"(h)
+        : "r"(byte & 255u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+__device__ __forceinline__ void e2m1x8_floats(unsigned word, float v[8])
+{
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const float2 f = e2m1x2_floats(word >> (8 * k));
+        v[2 * k] = f.x;
+        v[2 * k + 1] = f.y;
+    }
+}
+
+template <int DEG>
+__device__ __forceinline__ void mx4_codes(const unsigned (&w)[mx4_words(DEG)],
+                                          float (&q)[3 * mx4_rest(DEG) + 1])
+{
+    constexpr int E = 3 * mx4_rest(DEG), W = mx4_words(DEG);
+    if constexpr (DEG > 0) {
+        float v[8];
+        e2m1x8_floats(w[2], v);
+#pragma unroll
+        for (int j = 0; j < 6; j++) q[j] = v[j + 2];  // byte 0 is a scale
+#pragma unroll
+        for (int k = 3; k < W; k++) {
+            e2m1x8_floats(w[k], v);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (6 + 8 * (k - 3) + j < E) q[6 + 8 * (k - 3) + j] = v[j];
+        }
+    }
 }
 
 template <int W>
@@ -250,20 +288,6 @@ __device__ __forceinline__ float mx4_color(int use, const ShDir& D, float dc, fl
                       kSH_C4[8] * (xx * (xx - 3.f * yy) - yy * (3.f * xx - yy)) * r(23));
     }
     return v;
-}
-
-// The degree-4 basis values; sh_rest_basis (msp_math.cuh) has degrees 1-3.
-__device__ __forceinline__ void sh_rest_basis4(const ShDir& D, float* bs)
-{
-    bs[0] = kSH_C4[0] * D.xy * (D.xx - D.yy);
-    bs[1] = kSH_C4[1] * D.yz * (3.f * D.xx - D.yy);
-    bs[2] = kSH_C4[2] * D.xy * (7.f * D.zz - 1.f);
-    bs[3] = kSH_C4[3] * D.yz * (7.f * D.zz - 3.f);
-    bs[4] = kSH_C4[4] * (D.zz * (35.f * D.zz - 30.f) + 3.f);
-    bs[5] = kSH_C4[5] * D.xz * (7.f * D.zz - 3.f);
-    bs[6] = kSH_C4[6] * (D.xx - D.yy) * (7.f * D.zz - 1.f);
-    bs[7] = kSH_C4[7] * D.xz * (D.xx - 3.f * D.yy);
-    bs[8] = kSH_C4[8] * (D.xx * (D.xx - 3.f * D.yy) - D.yy * (3.f * D.xx - D.yy));
 }
 
 }  // namespace msp

@@ -143,21 +143,23 @@ def basis(means: np.ndarray, cam, use: int):
 
 # Roundings of one term of a basis value: the difference from the camera (1),
 # the norm's square (3 products and sums) and root (halved, rounded), its
-# reciprocal, and the product with the difference: 1 + (2 + 3) / 2 + 1 + 1 + 1
-# < 7 per factor of the direction, at most 4 factors; the constant's float and
-# the products and sums of the polynomial, at most 10.
+# reciprocal (2 with a Newton step), and the product with the difference:
+# 1 + (2 + 3) / 2 + 2 + 1 < 7 per factor of the direction, at most 4 factors;
+# the constant's float and the products and sums of the polynomial, at most
+# 10.
 BASIS_ROUNDINGS = 4 * 7 + 10
 
 
 def colors(dc, rest, means, cams, use: int):
-    """(colours, bounds) [V, n, 3]: each coefficient's product rounds once, a
-    degree's sum up to 9 times, the degrees' sums and the scale 5 times."""
+    """(colours, bounds) [V, n, 3]: a fused multiply-add per coefficient rounds
+    the sum at most 24 times, the dc term rounds once and joining it under
+    the scale once."""
     coef = np.concatenate((dc[:, None], rest[:, :REST[use]]), 1)
     col, bound = [], []
     for cam in cams:
         b, m = basis(means, cam, use)
         col.append(np.einsum("nk,nkc->nc", b, coef))
-        bound.append((BASIS_ROUNDINGS + 15) * U * np.einsum("nk,nkc->nc", m, np.abs(coef)))
+        bound.append((BASIS_ROUNDINGS + 26) * U * np.einsum("nk,nkc->nc", m, np.abs(coef)))
     shape = (len(cams), len(means), 3)
     return np.reshape(col, shape), np.reshape(bound, shape)
 

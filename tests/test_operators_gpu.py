@@ -156,6 +156,24 @@ def test_pack_unpack(n, degree):
     np.testing.assert_array_equal(host(grest), wrest)
 
 
+@pytest.mark.parametrize("degree", range(5))
+def test_unpack_every_byte(degree):
+    """Records of arbitrary bytes: each value of each byte, whether this
+    library would write it or not (scales from 2^-127 on; 255 is NaN)."""
+    rng = np.random.default_rng(degree)
+    rec = rng.integers(0, 256, (6000, oc.BYTES[degree]), dtype=np.uint8)
+    rec[:, 1] &= 0xBF                                 # halves that are finite numbers
+    rec[:, 3] &= 0xBF
+    rec[:, 5] &= 0xBF
+    if degree:
+        rec[:, 6:9] = rng.integers(0, 253, (6000, 3))
+        rec[:7, 6:9] = [[0, 1, 2], [252, 251, 250], [255, 0, 0], [0, 255, 0], [0, 0, 255], [255] * 3, [0] * 3]
+    gdc, grest = operators.mx4_unpack(dev(rec), degree)
+    wdc, wrest = oc.decode(rec, degree)
+    np.testing.assert_array_equal(host(gdc), wdc)
+    np.testing.assert_array_equal(host(grest), wrest)
+
+
 @pytest.mark.parametrize("degree", range(1, 5))
 def test_pack_awkward_values(degree):
     dc, rest = oc.awkward_features(degree)

@@ -104,8 +104,13 @@ def test_render_mx4_is_the_render_of_the_unpacked_scene(n, w, h, degree, use, kw
         for k in want:
             np.testing.assert_array_equal(got[k], want[k], err_msg=k)
     assert want["vis"].any()
+    # the colours of the same view as an operator: both within their bound of
+    # the exact ones (the renderer's unfused sums round twice as often)
+    vis = want["vis"]
     col = packed.colors(np.array([cs.cam_pos]), degrees_to_use=use)[0].cpu().numpy()
-    np.testing.assert_array_equal(col[want["vis"]], want["rgb"])
+    exact, bound = oc.colors(*oc.decode(packed.records.cpu().numpy(), degree), g.means, [cs.cam_pos], use)
+    assert (np.abs(col - exact[0]) <= bound[0]).all()
+    assert (np.abs(want["rgb"] - exact[0][vis]) <= 2 * bound[0][vis]).all()
     fdc, frest = packed.features()
     np.testing.assert_array_equal(fdc.cpu().numpy(), plain.params[3].cpu().numpy())
     np.testing.assert_array_equal(frest.cpu().numpy(), plain.params[4].cpu().numpy())
