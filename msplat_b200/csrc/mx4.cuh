@@ -70,11 +70,6 @@ __device__ __forceinline__ int mx4_scale_byte(unsigned amax)
     return min(252, max(0, (int)((amax + 0x200000u) >> 23) - 2));
 }
 
-__device__ __forceinline__ float mx4_scale(int byte)
-{
-    return __int_as_float(byte == 255 ? 0x7fc00000 : byte == 0 ? 0x00400000 : byte << 23);
-}
-
 // Encodes dc[3] and a row of rest coefficients.
 template <int DEG>
 __device__ __forceinline__ void mx4_encode(const float* dc, const float* row,
@@ -121,6 +116,7 @@ __device__ __forceinline__ void mx4_encode(const float* dc, const float* row,
 // first and narrowed from 32 bits: with the word unpacked into four byte
 // registers, or the byte narrowed from 16 bits, this compiler (12.9) reads the
 // wrong byte where some of a word's bytes are not used.
+// `byte` in 0..255.
 __device__ __forceinline__ float2 e2m1x2_floats(unsigned byte)
 {
     unsigned h;
@@ -130,7 +126,7 @@ __device__ __forceinline__ float2 e2m1x2_floats(unsigned byte)
         "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
         "}"
         : "=r"(h)
-        : "r"(byte & 255u));
+        : "r"(byte));
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
@@ -138,7 +134,7 @@ __device__ __forceinline__ void e2m1x8_floats(unsigned word, float v[8])
 {
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        const float2 f = e2m1x2_floats(word >> (8 * k));
+        const float2 f = e2m1x2_floats(__byte_perm(word, 0u, 0x4440u + k));
         v[2 * k] = f.x;
         v[2 * k + 1] = f.y;
     }
@@ -172,12 +168,22 @@ __device__ __forceinline__ void mx4_dc(const unsigned (&w)[W], float dc[3])
     dc[2] = __half2float(__ushort_as_half((unsigned short)w[1]));
 }
 
+// The scales 2^(b - 127) of r, g, b (b = 0: the subnormal 2^-127; 255: NaN):
+// two bytes to two bf16, which are the upper halves of floats.
+__device__ __forceinline__ float2 e8m0x2_floats(unsigned bytes)
+{
+    unsigned h;
+    asm("cvt.rn.bf16x2.ue8m0x2 %0, %1;" : "=r"(h) : "h"((unsigned short)bytes));
+    return make_float2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u));
+}
+
 template <int W>
 __device__ __forceinline__ void mx4_scales(const unsigned (&w)[W], float s[3])
 {
-    s[0] = mx4_scale((int)(w[1] >> 16 & 255u));
-    s[1] = mx4_scale((int)(w[1] >> 24));
-    s[2] = mx4_scale((int)(w[2] & 255u));
+    const float2 rg = e8m0x2_floats(w[1] >> 16);
+    s[0] = rg.x;
+    s[1] = rg.y;
+    s[2] = e8m0x2_floats(w[2] & 255u).x;
 }
 
 template <int DEG>
