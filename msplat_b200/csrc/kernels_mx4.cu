@@ -8,22 +8,26 @@
 namespace msp {
 namespace {
 
+// 224 bytes a Gaussian at degree 3 each, bound by memory.
 template <int DEG>
 __global__ void __launch_bounds__(kMxThreads)
 mx4_pack_kernel(int n, const float* __restrict__ dc, const float* __restrict__ rest,
                 void* __restrict__ records)
 {
-    constexpr int E = 3 * mx4_rest(DEG), PITCH = mx4_pitch<DEG>();
-    __shared__ float s_dc[kMxThreads * 3];
-    __shared__ float s_rest[E ? kMxThreads * PITCH : 1];
+    constexpr int E = 3 * mx4_rest(DEG), P = row_pitch(E);
+    __shared__ __align__(16) float s_dc[kMxThreads * 3];
+    __shared__ __align__(16) float s_rest[E ? kMxThreads * P : 4];
     const long long base = (long long)blockIdx.x * kMxThreads;
     const int cnt = (int)min((long long)kMxThreads, n - base);
-    rows_in<3, 3>(s_dc, dc + base * 3, cnt);
-    if constexpr (E > 0) rows_in<E, PITCH>(s_rest, rest + base * E, cnt);
+    if constexpr (E > 0) rows_in<E>(s_rest, rest + base * E, cnt);
+    rows_in<3>(s_dc, dc + base * 3, cnt);
+    rows_wait();
     __syncthreads();
     if (threadIdx.x >= cnt) return;
+    float q[E + 1];
+    if constexpr (E > 0) row_get<E>(s_rest + threadIdx.x * P, q);
     unsigned w[mx4_words(DEG)];
-    mx4_encode<DEG>(s_dc + 3 * threadIdx.x, s_rest + threadIdx.x * (E ? PITCH : 0), w);
+    mx4_encode<DEG>(s_dc + 3 * threadIdx.x, q, w);
     mx4_store<DEG>(records, base + threadIdx.x, w);
 }
 
@@ -32,9 +36,9 @@ __global__ void __launch_bounds__(kMxThreads)
 mx4_unpack_kernel(int n, const void* __restrict__ records, float* __restrict__ dc,
                   float* __restrict__ rest)
 {
-    constexpr int E = 3 * mx4_rest(DEG), PITCH = mx4_pitch<DEG>();
-    __shared__ float s_dc[kMxThreads * 3];
-    __shared__ float s_rest[E ? kMxThreads * PITCH : 1];
+    constexpr int E = 3 * mx4_rest(DEG), P = row_pitch(E);
+    __shared__ __align__(16) float s_dc[kMxThreads * 3];
+    __shared__ __align__(16) float s_rest[E ? kMxThreads * P : 4];
     const long long base = (long long)blockIdx.x * kMxThreads;
     const int cnt = (int)min((long long)kMxThreads, n - base);
     if (threadIdx.x < cnt) {
@@ -46,12 +50,15 @@ mx4_unpack_kernel(int n, const void* __restrict__ records, float* __restrict__ d
             mx4_scales(w, s);
             mx4_codes<DEG>(w, q);
 #pragma unroll
-            for (int j = 0; j < E; j++) s_rest[threadIdx.x * PITCH + j] = q[j] * s[j % 3];
+            for (int j = 0; j < E; j++) q[j] *= s[j % 3];
+            row_put<E>(s_rest + threadIdx.x * P, q);
         }
     }
+    rows_done();
     __syncthreads();
-    rows_out<3, 3>(dc + base * 3, s_dc, cnt);
-    if constexpr (E > 0) rows_out<E, PITCH>(rest + base * E, s_rest, cnt);
+    if constexpr (E > 0) rows_out<E>(rest + base * E, s_rest, cnt);
+    rows_out<3>(dc + base * 3, s_dc, cnt);
+    rows_left();
 }
 
 // One view's colours of the visible Gaussians, into the renderer's buffer.

@@ -156,17 +156,17 @@ mx4_colors_backward_kernel(int n, const float* __restrict__ means, int views, co
                            const int* __restrict__ radii, const float* __restrict__ v_colors,
                            float* __restrict__ v_dc, float* __restrict__ v_rest)
 {
-    constexpr int B = mx4_rest(USE), E = 3 * mx4_rest(DEG), PITCH = mx4_pitch<DEG>();
-    __shared__ float s_dc[kMxThreads * 3];
-    __shared__ float s_rest[E ? kMxThreads * PITCH : 1];
+    constexpr int B = mx4_rest(USE), E = 3 * mx4_rest(DEG), P = row_pitch(E);
+    __shared__ __align__(16) float s_dc[kMxThreads * 3];
+    __shared__ __align__(16) float s_rest[E ? kMxThreads * P : 4];
     const long long base = (long long)blockIdx.x * kMxThreads;
     const long long i = base + threadIdx.x;
     const int cnt = (int)min((long long)kMxThreads, n - base);
     if (i < n) {
         const unsigned long long seen = views > 0 ? views_of(radii, i, n, views) : 0ull;
-        float gd[3] = {0.f, 0.f, 0.f}, gr[3 * B + 1];
+        float gd[3] = {0.f, 0.f, 0.f}, gr[E + 1];  // rows of degrees not in use stay 0
 #pragma unroll
-        for (int e = 0; e < 3 * B; e++) gr[e] = 0.f;
+        for (int e = 0; e < E; e++) gr[e] = 0.f;
         float p[3];
 #pragma unroll
         for (int k = 0; k < 3; k++) p[k] = means[3 * i + k];
@@ -190,12 +190,13 @@ mx4_colors_backward_kernel(int n, const float* __restrict__ means, int views, co
         }
 #pragma unroll
         for (int c = 0; c < 3; c++) s_dc[3 * threadIdx.x + c] = MSP_SH_C0 * gd[c];
-#pragma unroll
-        for (int e = 0; e < E; e++) s_rest[threadIdx.x * PITCH + e] = e < 3 * B ? gr[e < 3 * B ? e : 0] : 0.f;
+        if constexpr (E > 0) row_put<E>(s_rest + threadIdx.x * P, gr);
     }
+    rows_done();
     __syncthreads();
-    rows_out<3, 3>(v_dc + base * 3, s_dc, cnt);
-    if constexpr (E > 0) rows_out<E, PITCH>(v_rest + base * E, s_rest, cnt);
+    if constexpr (E > 0) rows_out<E>(v_rest + base * E, s_rest, cnt);
+    rows_out<3>(v_dc + base * 3, s_dc, cnt);
+    rows_left();
 }
 
 bool views_ok(const char* who, int degree, int degrees_to_use, int views, const float* cam_pos,

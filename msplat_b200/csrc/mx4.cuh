@@ -70,9 +70,9 @@ __device__ __forceinline__ int mx4_scale_byte(unsigned amax)
     return min(252, max(0, (int)((amax + 0x200000u) >> 23) - 2));
 }
 
-// Encodes dc[3] and a row of rest coefficients.
+// Encodes dc[3] and a row q of rest coefficients, which it scales in place.
 template <int DEG>
-__device__ __forceinline__ void mx4_encode(const float* dc, const float* row,
+__device__ __forceinline__ void mx4_encode(const float* dc, float (&q)[3 * mx4_rest(DEG) + 1],
                                            unsigned (&w)[mx4_words(DEG)])
 {
     constexpr int E = 3 * mx4_rest(DEG), W = mx4_words(DEG);
@@ -82,13 +82,10 @@ __device__ __forceinline__ void mx4_encode(const float* dc, const float* row,
     w[0] = h0 | h1 << 16;
     w[1] = h2;
     if constexpr (DEG > 0) {
-        float q[E];
         unsigned top[3] = {0u, 0u, 0u};
 #pragma unroll
-        for (int j = 0; j < E; j++) {
-            q[j] = row[j];
+        for (int j = 0; j < E; j++)
             top[j % 3] = max(top[j % 3], __float_as_uint(q[j]) & 0x7fffffffu);
-        }
         int b[3];
         float inv[3];
 #pragma unroll
