@@ -81,7 +81,7 @@ __device__ __forceinline__ unsigned long long views_of(const int* radii, long lo
 // that coefficients are decoded as they are multiplied and not held.
 // One view of 1M Gaussians, 60% visible: 14.9 us with G = 2 (17.5 with 1, 17.0
 // with 4); 8 views of 6M: 260 us with G = 1, 2 (107 registers) no faster.
-template <int DEG, int USE, bool ONE, int G>
+template <int DEG, int USE, bool ONE, int G, bool MASKED>
 __global__ void __launch_bounds__(kMxThreads)
 mx4_colors_kernel(int n, const float* __restrict__ means, const void* __restrict__ records,
                   int views_arg, const Mx4Cams cams, const int* __restrict__ radii,
@@ -95,10 +95,12 @@ mx4_colors_kernel(int n, const float* __restrict__ means, const void* __restrict
     unsigned long long seen[G];
     float p[G][3];
     unsigned w[G][mx4_words(DEG)];
+    int left[G];  // floats of the warp's rows that exist
 #pragma unroll
     for (int g = 0; g < G; g++) {
+        left[g] = (int)min(96LL, max(0LL, 3 * (n - (base + g * kMxThreads + w0))));
         const long long i = base + g * kMxThreads + tid;
-        seen[g] = i < n ? views_of(radii, i, n, views) : 0ull;
+        seen[g] = i >= n ? 0ull : MASKED ? views_of(radii, i, n, views) : ~0ull;
     }
 #pragma unroll
     for (int g = 0; g < G; g++) {
@@ -119,8 +121,8 @@ mx4_colors_kernel(int n, const float* __restrict__ means, const void* __restrict
             mx4_codes<DEG>(w[g], q);
         }
         for (int v = 0; v < views; v++) {
-            const bool on = (seen[g] >> v) & 1ull;
-            if (on) {
+            const bool on = MASKED ? (seen[g] >> v) & 1ull : seen[g] != 0;
+            if (on || !MASKED) {
                 float col[3] = {dc[0], dc[1], dc[2]};
                 if constexpr (USE > 0) {
                     float d[3], b[B];
@@ -137,13 +139,13 @@ mx4_colors_kernel(int n, const float* __restrict__ means, const void* __restrict
 #pragma unroll
                 for (int c = 0; c < 3; c++) s_col[3 * tid + c] = col[c];
             }
-            const unsigned bal = __ballot_sync(0xffffffffu, on);
+            const unsigned bal = MASKED ? __ballot_sync(0xffffffffu, on) : 0u;
             __syncwarp();
             float* out = colors + (v * (long long)n + base + g * kMxThreads + w0) * 3;
 #pragma unroll
             for (int k = 0; k < 3; k++) {
                 const int e = 32 * k + lane;
-                if ((bal >> (e / 3)) & 1u) out[e] = s_col[3 * w0 + e];
+                if (MASKED ? (bal >> (e / 3)) & 1u : e < left[g]) out[e] = s_col[3 * w0 + e];
             }
             __syncwarp();
         }
@@ -249,8 +251,13 @@ int msplat_mx4_colors(int n, int degree, int degrees_to_use, const float* means3
             kernel<<<(unsigned)(((long long)n + per - 1) / per), kMxThreads, 0, st>>>(
                 n, means3d, records, num_views, cams, radii, colors);
         };
-        num_views == 1 ? run(mx4_colors_kernel<D.value, U.value, true, 2>, 2 * kMxThreads)
-                       : run(mx4_colors_kernel<D.value, U.value, false, 1>, kMxThreads);
+        constexpr int d = D.value, u = U.value;
+        if (num_views == 1)
+            radii ? run(mx4_colors_kernel<d, u, true, 2, true>, 2 * kMxThreads)
+                  : run(mx4_colors_kernel<d, u, true, 2, false>, 2 * kMxThreads);
+        else
+            radii ? run(mx4_colors_kernel<d, u, false, 1, true>, kMxThreads)
+                  : run(mx4_colors_kernel<d, u, false, 1, false>, kMxThreads);
     });
     return launched(who, 1);
 }
