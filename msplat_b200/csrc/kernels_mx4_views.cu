@@ -2,6 +2,8 @@
 // (format in mx4.cuh) and the gradient of the coefficients.  Compiled with FMA
 // contraction: a fused multiply-add per coefficient and view is what bounds
 // many views.  (A renderer's view, kernels_mx4.cu, keeps the projection's bits.)
+#include <algorithm>
+
 #include "mx4_rows.cuh"
 
 namespace msp {
@@ -80,84 +82,161 @@ __device__ __forceinline__ unsigned long long views_of(const int* radii, long lo
     return seen;
 }
 
-// Colours of Gaussians [base, base + G * kMxThreads), G of them a thread: the
-// loads of all of them are under way before the first is decoded.
-// DEG: the records' degree; USE: the degrees in use; ONE: a single view, so
-// that coefficients are decoded as they are multiplied and not held.
-// One view of 1M Gaussians, 60% visible: 14.9 us with G = 2 (17.5 with 1, 17.0
-// with 4); 8 views of 6M: 260 us with G = 1, 2 (107 registers) no faster.
-template <int DEG, int USE, bool ONE, int G, bool MASKED>
-__global__ void __launch_bounds__(kMxThreads)
-mx4_colors_kernel(int n, const float* __restrict__ means, const void* __restrict__ records,
-                  int views_arg, const Mx4Cams cams, const int* __restrict__ radii,
-                  float* __restrict__ colors)
+// What a thread needs of one Gaussian, as it comes from memory.
+template <int DEG>
+struct RawGaussian {
+    float p[3];
+    unsigned w[mx4_words(DEG)];
+    __device__ __forceinline__ void load(const float* means, const void* records, long long i)
+    {
+#pragma unroll
+        for (int k = 0; k < 3; k++) p[k] = means[3 * i + k];
+        mx4_load<DEG>(records, i, w);
+    }
+};
+
+// The colour of one view.
+template <int USE>
+__device__ __forceinline__ void color_of(const float* cam, const float p[3], const float* q,
+                                         const float s[3], const float dc[3], float col[3])
+{
+#pragma unroll
+    for (int c = 0; c < 3; c++) col[c] = dc[c];
+    if constexpr (USE > 0) {
+        constexpr int B = mx4_rest(USE);
+        float d[3], b[B];
+        unit_dir(cam, p, d);
+        sh_basis<USE>(d, b);
+#pragma unroll
+        for (int c = 0; c < 3; c++) {
+            float sum = b[0] * q[c];
+#pragma unroll
+            for (int k = 1; k < B; k++) sum = fmaf(b[k], q[3 * k + c], sum);
+            col[c] = fmaf(s[c], sum, dc[c]);
+        }
+    }
+}
+
+// The same, decoding the record as it goes: eight coefficients at a time are
+// held and not all of them.
+template <int DEG, int USE>
+__device__ __forceinline__ void color_of_record(const float* cam, const RawGaussian<DEG>& g, float col[3])
 {
     constexpr int B = mx4_rest(USE);
-    const int views = ONE ? 1 : views_arg;
-    __shared__ float s_col[kMxThreads * 3];
+    mx4_dc(g.w, col);
+#pragma unroll
+    for (int c = 0; c < 3; c++) col[c] *= MSP_SH_C0;
+    if constexpr (USE > 0) {
+        float d[3], b[B], s[3], sum[3];
+        mx4_scales(g.w, s);
+        unit_dir(cam, g.p, d);
+        sh_basis<USE>(d, b);
+#pragma unroll
+        for (int k = 2; k < mx4_words(DEG); k++) {
+            float v[8];
+            e2m1x8_floats(g.w[k], v);
+#pragma unroll
+            for (int h = 0; h < 8; h++) {
+                const int j = 8 * k + h - 18;  // bytes 0-8 of the record are 18 codes' room
+                if (j < 0 || j >= 3 * B) continue;
+                sum[j % 3] = j < 3 ? b[0] * v[h] : fmaf(b[j / 3], v[h], sum[j % 3]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 3; c++) col[c] = fmaf(s[c], sum[c], col[c]);
+    }
+}
+
+// A warp's 32 colours through shared memory to `out` (its first Gaussian's):
+// of those in `mask`, or with ALL the first `left` floats.
+template <bool ALL>
+__device__ __forceinline__ void put_colors(float* out, float* s_col, const float col[3],
+                                           unsigned mask, int left)
+{
     const int tid = threadIdx.x, lane = tid & 31, w0 = tid & ~31;
-    const long long base = (long long)blockIdx.x * (kMxThreads * G);
-    unsigned long long seen[G];
-    float p[G][3];
-    unsigned w[G][mx4_words(DEG)];
-    int left[G];  // floats of the warp's rows that exist
 #pragma unroll
-    for (int g = 0; g < G; g++) {
-        left[g] = (int)min(96LL, max(0LL, 3 * (n - (base + g * kMxThreads + w0))));
-        const long long i = base + g * kMxThreads + tid;
-        // One view reads what it sees only; of several, most Gaussians have
-        // one that sees them, and their loads need not wait for the masks.
-        if (MASKED && ONE) seen[g] = i < n ? views_of(radii, i, n, 1) : 0ull;
-        else seen[g] = i < n ? ~0ull : 0ull;
+    for (int c = 0; c < 3; c++) s_col[3 * tid + c] = col[c];
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+        const int e = 32 * k + lane;
+        if (ALL ? e < left : (mask >> (e / 3)) & 1u) out[e] = s_col[3 * w0 + e];
     }
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        const long long i = base + g * kMxThreads + tid;
-        if (!seen[g]) continue;
-#pragma unroll
-        for (int k = 0; k < 3; k++) p[g][k] = means[3 * i + k];
-        mx4_load<DEG>(records, i, w[g]);
-        if (MASKED && !ONE) seen[g] = views_of(radii, i, n, views);
+    __syncwarp();
+}
+
+// Floats of a warp's colours that exist when its first Gaussian is i0.
+__device__ __forceinline__ int floats_left(long long n, long long i0)
+{
+    return (int)min(96LL, max(0LL, 3 * (n - i0)));
+}
+
+// One view.  Blocks stay and take every gridDim-th tile of kMxThreads
+// Gaussians; a tile's records load while the one before is computed, and its
+// radii, which say what of them to load, one tile earlier still.  1M Gaussians,
+// 60% visible: 13.7 us (a block per 256 Gaussians, all loads up front: 15.1; per
+// 128: 17.5).  Degree 4 would spill at the other degrees' 64 registers.
+constexpr int one_view_blocks(int deg) { return deg == 4 ? 6 : 8; }
+template <int DEG, int USE, bool MASKED>
+__global__ void __launch_bounds__(kMxThreads, one_view_blocks(DEG))
+mx4_colors_one_kernel(int n, const float* __restrict__ means, const void* __restrict__ records,
+                      int, const Mx4Cams cams, const int* __restrict__ radii,
+                      float* __restrict__ colors)
+{
+    __shared__ float s_col[kMxThreads * 3];
+    const long long step = (long long)gridDim.x * kMxThreads;
+    long long i = (long long)blockIdx.x * kMxThreads + threadIdx.x;
+    auto visible = [&](long long j) { return j < n && (!MASKED || radii[j] > 0); };
+    bool on = visible(i), on_next = visible(i + step);
+    RawGaussian<DEG> g, g_next;
+    if (on) g.load(means, records, i);
+    for (; i - threadIdx.x < n; i += step) {
+        const bool on_after = visible(i + 2 * step);
+        if (on_next) g_next.load(means, records, i + step);
+        float col[3];
+        color_of_record<DEG, USE>(cams.p[0], g, col);
+        const long long i0 = i - (threadIdx.x & 31);
+        const unsigned mask = MASKED ? __ballot_sync(0xffffffffu, on) : 0u;
+        put_colors<!MASKED>(colors + 3 * i0, s_col, col, mask, floats_left(n, i0));
+        g = g_next;
+        on = on_next;
+        on_next = on_after;
     }
+}
+
+// Several views, one Gaussian a thread, its coefficients decoded once.  Bound
+// by arithmetic: at degree 3 about a hundred operations a colour.  8 views of
+// 6M Gaussians: 233 us (a pair of Gaussians a thread with the two-float
+// instructions: 226 to 261, their rate is the same).
+template <int DEG, int USE, bool MASKED>
+__global__ void __launch_bounds__(kMxThreads)
+mx4_colors_kernel(int n, const float* __restrict__ means, const void* __restrict__ records,
+                  int views, const Mx4Cams cams, const int* __restrict__ radii,
+                  float* __restrict__ colors)
+{
+    __shared__ float s_col[kMxThreads * 3];
+    const long long i = (long long)blockIdx.x * kMxThreads + threadIdx.x;
+    const long long i0 = i - (threadIdx.x & 31);
+    const int left = floats_left(n, i0);
+    unsigned long long seen = 0;
+    RawGaussian<DEG> g;
+    if (i < n) {  // most Gaussians have a view that sees them: no wait for the masks
+        g.load(means, records, i);
+        seen = MASKED ? views_of(radii, i, n, views) : ~0ull;
+    }
+    float dc[3], s[3], q[3 * mx4_rest(DEG) + 1], col[3];
+    mx4_dc(g.w, dc);
 #pragma unroll
-    for (int g = 0; g < G; g++) {
-        float dc[3], s[3], q[3 * mx4_rest(DEG) + 1];
-        mx4_dc(w[g], dc);
-#pragma unroll
-        for (int c = 0; c < 3; c++) dc[c] *= MSP_SH_C0;
-        if constexpr (USE > 0) {
-            mx4_scales(w[g], s);
-            mx4_codes<DEG>(w[g], q);
-        }
-        for (int v = 0; v < views; v++) {
-            const bool on = MASKED ? (seen[g] >> v) & 1ull : seen[g] != 0;
-            if (on || !MASKED) {
-                float col[3] = {dc[0], dc[1], dc[2]};
-                if constexpr (USE > 0) {
-                    float d[3], b[B];
-                    unit_dir(cams.p[v], p[g], d);
-                    sh_basis<USE>(d, b);
-#pragma unroll
-                    for (int c = 0; c < 3; c++) {
-                        float sum = b[0] * q[c];
-#pragma unroll
-                        for (int k = 1; k < B; k++) sum = fmaf(b[k], q[3 * k + c], sum);
-                        col[c] = fmaf(s[c], sum, dc[c]);
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < 3; c++) s_col[3 * tid + c] = col[c];
-            }
-            const unsigned bal = MASKED ? __ballot_sync(0xffffffffu, on) : 0u;
-            __syncwarp();
-            float* out = colors + (v * (long long)n + base + g * kMxThreads + w0) * 3;
-#pragma unroll
-            for (int k = 0; k < 3; k++) {
-                const int e = 32 * k + lane;
-                if (MASKED ? (bal >> (e / 3)) & 1u : e < left[g]) out[e] = s_col[3 * w0 + e];
-            }
-            __syncwarp();
-        }
+    for (int c = 0; c < 3; c++) dc[c] *= MSP_SH_C0;
+    if constexpr (USE > 0) {
+        mx4_scales(g.w, s);
+        mx4_codes<DEG>(g.w, q);
+    }
+    for (int v = 0; v < views; v++) {
+        const bool on = (seen >> v) & 1ull;
+        if (!MASKED || on) color_of<USE>(cams.p[v], g.p, q, s, dc, col);
+        const unsigned mask = MASKED ? __ballot_sync(0xffffffffu, on) : 0u;
+        put_colors<!MASKED>(colors + 3 * (v * (long long)n + i0), s_col, col, mask, left);
     }
 }
 
@@ -267,17 +346,17 @@ int msplat_mx4_colors(int n, int degree, int degrees_to_use, const float* means3
     if (!mx4_records_ok(who, records, degree)) return MSPLAT_ERR_ARG;
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     with_degrees(degree, degrees_to_use, [&](auto D, auto U) {
-        auto run = [&](auto kernel, int per) {
-            kernel<<<(unsigned)(((long long)n + per - 1) / per), kMxThreads, 0, st>>>(
-                n, means3d, records, num_views, cams, radii, colors);
-        };
         constexpr int d = D.value, u = U.value;
+        auto run = [&](auto kernel, unsigned blocks) {
+            kernel<<<blocks, kMxThreads, 0, st>>>(n, means3d, records, num_views, cams, radii, colors);
+        };
+        const unsigned tiles = mx4_blocks(n), stay = std::min(tiles, 148u * one_view_blocks(d));
         if (num_views == 1)
-            radii ? run(mx4_colors_kernel<d, u, true, 2, true>, 2 * kMxThreads)
-                  : run(mx4_colors_kernel<d, u, true, 2, false>, 2 * kMxThreads);
+            radii ? run(mx4_colors_one_kernel<d, u, true>, stay)
+                  : run(mx4_colors_one_kernel<d, u, false>, stay);
         else
-            radii ? run(mx4_colors_kernel<d, u, false, 1, true>, kMxThreads)
-                  : run(mx4_colors_kernel<d, u, false, 1, false>, kMxThreads);
+            radii ? run(mx4_colors_kernel<d, u, true>, tiles)
+                  : run(mx4_colors_kernel<d, u, false>, tiles);
     });
     return launched(who, 1);
 }
