@@ -69,7 +69,6 @@ struct Engine {
     bool user_stream_set = false;
     // allocated sizes
     long long cap_N = 0, cap_grad_N = 0, cap_pix = 0, cap_T = 0, cap_isect = 0, cap_chunk = 0;
-    size_t cap_records = 0;  // bytes
     StepOptions opt;
     Buffers B{};
     ParamSlot* d_slot = nullptr;
@@ -212,7 +211,7 @@ static void free_buffers()
                     B.proj.sh_mean, B.tile_count, B.tile_offset, B.tile_order, B.tile_sorted, B.tile_flag, B.keys, B.keys_alt,
                     B.sorted_ids, B.out_img,
                     B.final_T, B.final_idx, B.v_rendered, B.grad_acc,
-                    B.chunk_T, B.chunk_C, B.chunk_idx, B.prefix_T, B.after_C, B.records};
+                    B.chunk_T, B.chunk_C, B.chunk_idx, B.prefix_T, B.after_C};
     for (void* p : ptrs)
         if (p) cudaFree(p);
     float* ls = B.loss_sum;
@@ -225,7 +224,6 @@ static void free_buffers()
     B.isect_total = it;
     B.max_tile = mt;
     g.cap_N = g.cap_grad_N = g.cap_pix = g.cap_T = g.cap_isect = g.cap_chunk = 0;
-    g.cap_records = 0;
 }
 
 // Buffer cache: grow-only, like FusedTensorCache::ensure_* (msplat_metal.mm:383-452).
@@ -439,60 +437,20 @@ static int dense_bins_for(const StepParams& p)
     return (g.last_isect_n > 0 && g.last_isect > (long long)kDenseRatio * g.last_isect_n) ? 1 : 0;
 }
 
-// Room for this step's records (training with 4-bit colours).
-static int ensure_records(size_t bytes)
-{
-    if (bytes <= g.cap_records) return MSPLAT_OK;
-    if (g.B.records) cudaFree(g.B.records);
-    g.B.records = nullptr;
-    g.cap_records = 0;
-    MSP_CUDA(cudaMalloc(&g.B.records, bytes));
-    g.cap_records = bytes;
-    return MSPLAT_OK;
-}
-
-// The side stream, made to wait for everything queued on st so far; st
-// itself when the events fail.
-static cudaStream_t fork_side(cudaStream_t st)
-{
-    const bool forked = cudaEventRecord(g.side.fork, st) == cudaSuccess &&
-                        cudaStreamWaitEvent(g.side.stream, g.side.fork, 0) == cudaSuccess;
-    return forked ? g.side.stream : st;
-}
-
 // Forward half shared by render and train (forward_pipeline, msplat_metal.mm:462-750).
-// With `records` the colours come from them, on the side stream: binning and
-// sorting, which wait on latency and atomics more than on bandwidth, need
-// none, so the colours stream beside them and join before the raster.  With
-// `pack` the records are this step's, packed from dc and rest beside the
-// projection.
+// With `records` they hold the colours, and dc and rest are not read.
 static int run_forward(const StepParams& p, const float* means, const float* scales,
                        const float* quats, const float* dc, const float* rest, const float* opac,
-                       bool train, StageMarks& tm, cudaStream_t st, void* records = nullptr,
-                       bool pack = false)
+                       bool train, StageMarks& tm, cudaStream_t st, const void* records = nullptr)
 {
     const Buffers& B = g.B;
-    const bool dropout = train && g.opt.dropout;
+    const Colors colors = records ? Colors::kRecords
+                        : train && g.opt.mx4 ? Colors::kRounded : Colors::kFeatures;
     tm.mark(0, st);
-    cudaStream_t cs = st;
-    if (pack) {
-        cs = fork_side(st);
-        launch_mx4_pack(p.num_points, p.degree, dc, rest, records, cs);
-    }
-    launch_project_forward(g.d_params, p.num_points, means, scales, quats, dc, rest, opac, B, train,
-                           p.degrees_to_use, p.rest_stride, st, records == nullptr, dropout);
-    if (records) {
-        const cudaStream_t rs = fork_side(st);
-        if (rs != cs && pack) cudaStreamSynchronize(cs);  // an event failed: the records first
-        cs = rs;
-        launch_mx4_rgb(p.num_points, p.degree, p.degrees_to_use, means, records, p.cam_pos,
-                       B.proj.radii, B.proj.rgb, cs);
-        if (cs != st && cudaEventRecord(g.side.join, cs) != cudaSuccess) {
-            cudaStreamSynchronize(cs);
-            cs = st;
-        }
-        g.launches += 1 + pack;
-    }
+    launch_project_forward(g.d_params, p.num_points, means, scales, quats, dc,
+                           records ? static_cast<const float*>(records) : rest, opac, B, train,
+                           p.degrees_to_use, records ? mx4_words(p.degree) : p.rest_stride, st,
+                           colors, train && g.opt.dropout);
     tm.mark(1, st);
     launch_scan_tiles(g.d_params, p.num_tiles, p.dense_bins != 0, B, st);
     launch_scatter(g.d_params, p.num_points, B, st);
@@ -503,7 +461,6 @@ static int run_forward(const StepParams& p, const float* means, const float* sca
     const int sort_launches = launch_sort_tiles(g.d_params, p.num_tiles, p.prefix_sort != 0,
                                                 large_sort, huge_sort, B, st);
     tm.mark(2, st);
-    if (cs != st && cudaStreamWaitEvent(st, g.side.join, 0) != cudaSuccess) cudaStreamSynchronize(cs);
     launch_raster_forward(g.d_params, p.num_tiles, p.k_max, p.prefix_sort != 0, p.img_w, p.img_h, B,
                           st);
     g.last_k_max = p.k_max;
@@ -748,12 +705,11 @@ static int train_common(const char* who, int num_points, float* means3d, float* 
     p.drop_inv = (float)(1.0 - g.opt.threshold / 4294967296.0);
     const cudaStream_t st = g.stream();
     if ((rc = ensure(num_points, img_width, img_height, p.num_tiles, p.k_max, true))) return rc;
-    if (g.opt.mx4 && (rc = ensure_records((size_t)num_points * 4 * mx4_words(p.degree)))) return rc;
     p.capacity = g.cap_isect;
     StageMarks tm = begin_timing();
     if ((rc = upload_params(p, st))) return rc;
     if ((rc = run_forward(p, means3d, scales, quats, features_dc, features_rest, opacities, true,
-                          tm, st, g.opt.mx4 ? g.B.records : nullptr, g.opt.mx4)))
+                          tm, st)))
         return rc;
     tm.mark(3, st);
     launch_ssim(g.d_params, p.img_w, p.img_h, gt, g.B, st);
@@ -1001,7 +957,7 @@ static int render_common(int num_points, const float* means3d, const float* scal
                          unsigned img_height, unsigned img_width, const int* tile_bounds,
                          float clip_thresh, unsigned degree, unsigned degrees_to_use,
                          const float* cam_pos, const float* features_dc,
-                         const float* features_rest, void* records, const float* opacities,
+                         const float* features_rest, const void* records, const float* opacities,
                          const float* background, float** out_img)
 {
     std::lock_guard<std::mutex> lk(g_mu);
@@ -1063,7 +1019,7 @@ int msplat_render_mx4(int num_points, const float* means3d, const float* scales,
     if (num_points > 0 && !mx4_records_ok(who, records, (int)degree)) return MSPLAT_ERR_ARG;
     return render_common(num_points, means3d, scales, glob_scale, quats, viewmat, projmat, fx, fy,
                          cx, cy, img_height, img_width, tile_bounds, clip_thresh, degree,
-                         degrees_to_use, cam_pos, nullptr, nullptr, const_cast<void*>(records),
+                         degrees_to_use, cam_pos, nullptr, nullptr, records,
                          opacities, background, out_img);
 }
 

@@ -108,7 +108,6 @@ struct Buffers {
     int* chunk_idx;        // [K*H*W]
     float* prefix_T;       // [K*H*W]
     float* after_C;        // [K*H*W*3]
-    void* records;         // training with 4-bit colours only: this step's records
     float* loss_sum;       // [1]
     int* err;              // [1]
     int* isect_total;      // [1] intersections of the view (scan output), or null
@@ -229,17 +228,18 @@ void set_error(const char* fmt, ...);                  // text for msplat_last_e
 int fill_params(StepParams& p, const CamArgs& a);      // validates, fills the block
 int chunk_k_max(long long N, int num_tiles);           // depth chunks of one tile
 
+// Where a forward's colours come from: the features; the features rounded as
+// 4-bit records hold them; or records, which then stand in the place of the
+// SH-rest rows (`rest` their array, `rest_stride` their words).
+enum class Colors { kFeatures, kRounded, kRecords };
+
 // Kernel launchers (kernels_*.cu).
 void launch_project_forward(const StepParams* P, int N, const float* means, const float* scales,
                             const float* quats, const float* dc, const float* rest,
                             const float* opac, const Buffers& B, bool zero_grads,
                             int degrees_to_use_host, int rest_stride_host, cudaStream_t s,
-                            bool colors = true, bool dropout = false);
-// 4-bit colours (kernels_mx4.cu), for callers that checked the arguments.
-void launch_mx4_pack(int n, int degree, const float* dc, const float* rest, void* records,
-                     cudaStream_t s);
-void launch_mx4_rgb(int n, int degree, int use, const float* means, const void* records,
-                    const float* cam_pos, const int* radii, float4* rgb, cudaStream_t s);
+                            Colors colors = Colors::kFeatures, bool dropout = false);
+// Whether `records` can be a record array (kernels_mx4.cu); sets the error.
 bool mx4_records_ok(const char* who, const void* records, int degree);
 void launch_scan_tiles(const StepParams* P, int num_tiles, bool dense_bins, const Buffers& B,
                        cudaStream_t s);

@@ -232,7 +232,7 @@ extern "C" int msplat_dropout(long long rows, int cols, const float* x, long lon
     if (x_stride == 0) x_stride = cols;
     if (y_stride == 0) y_stride = cols;
     if (rows < 0 || cols < 1 || x_stride < cols || y_stride < cols ||
-        rows > (1LL << 60) / std::max(x_stride, y_stride)) {
+        rows > (1LL << 46) / std::max(x_stride, y_stride)) {
         set_error("msplat_dropout: invalid shape (%lld rows of %d, strides %lld and %lld)", rows,
                   cols, x_stride, y_stride);
         return MSPLAT_ERR_ARG;

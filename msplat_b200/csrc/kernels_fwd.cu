@@ -2,9 +2,12 @@
 // per-tile depth sort and the forward rasterizer.  Compiled with
 // --fmad=false (see msp_math.cuh): every value here is bit-identical to the
 // CPU oracle.
+#include <type_traits>
+
 #include "dropout.cuh"
 #include "engine.h"
 #include "msp_math.cuh"
+#include "mx4.cuh"
 #include "tma.cuh"
 
 namespace msp {
@@ -81,6 +84,9 @@ __device__ __forceinline__ void sh_to_color(int degree, float x, float y, float 
     }
 }
 
+template <int DEG>
+using Degree = std::integral_constant<int, DEG>;
+
 // Block layout of the staged inputs in shared memory (floats).
 struct ProjStage {
     static constexpr int kMeans = 0;
@@ -97,13 +103,18 @@ struct ProjStage {
 // block is full and the arrays are 16-byte aligned, else by plain loads.
 // Every byte of the block is then in flight at once instead of in two
 // dependent rounds (geometry, then the SH rows of the visible Gaussians).
-// Without COLORS the colours come from 4-bit records: dc and rest are
-// neither staged nor read, and out.rgb is left to another kernel.  With
-// DROPOUT a Gaussian that its draw drops is culled -- not binned, sorted,
+// COLORS (see engine.h): kRounded takes each staged row through its 4-bit
+// record (training: the same step time, 1.65 ms on 1M Gaussians and 4.21 on 6M;
+// packing records beside this kernel and reading them later took 0.03 and 0.17
+// ms more; six blocks a multiprocessor, at 128 bytes of spills: 0.02 ms of 6M's
+// step).  kRecords stages records instead of dc and rows: 76 of 236 bytes a
+// Gaussian at degree 3, a render of 6M in 1.50 ms (1.59 from features), of 1M in
+// 0.596 (0.615); by a kernel of their own on another stream, beside binning and
+// sorting, the colours took 1.52 and 0.587.  With DROPOUT a Gaussian that its draw drops is culled -- not binned, sorted,
 // blended nor given gradients -- and the others' opacity is multiplied by
 // drop_scale.
-template <bool ZERO_GRADS, bool COLORS, bool DROPOUT>
-__global__ void __launch_bounds__(kProjThreads)
+template <bool ZERO_GRADS, Colors COLORS, bool DROPOUT>
+__global__ void __launch_bounds__(kProjThreads, COLORS == Colors::kRounded ? 6 : 0)
 project_forward_kernel(const StepParams* __restrict__ P, int N, const float* __restrict__ means,
                        const float* __restrict__ scales, const float* __restrict__ quats,
                        const float* __restrict__ dc, const float* __restrict__ rest,
@@ -111,6 +122,7 @@ project_forward_kernel(const StepParams* __restrict__ P, int N, const float* __r
                        float* __restrict__ grad_acc, int rest_stride, int bulk,
                        int* __restrict__ err)
 {
+    constexpr bool kDc = COLORS != Colors::kRecords;  // dc is used
     extern __shared__ __align__(16) float sm[];
     __shared__ unsigned long long s_bar;
     __shared__ int s_fail;
@@ -130,13 +142,13 @@ project_forward_kernel(const StepParams* __restrict__ P, int N, const float* __r
         if (tid == 0) mbar_init(&s_bar);
         __syncthreads();
         if (tid == 0) {
-            const unsigned rs_bytes = COLORS ? (unsigned)(kProjThreads * rest_stride * 4) : 0u;
-            mbar_expect_tx(&s_bar, (unsigned)((COLORS ? ProjStage::kRest : ProjStage::kDc) * 4) + rs_bytes);
+            const unsigned rs_bytes = (unsigned)(kProjThreads * rest_stride * 4);
+            mbar_expect_tx(&s_bar, (unsigned)((kDc ? ProjStage::kRest : ProjStage::kDc) * 4) + rs_bytes);
             bulk_load(sm + ProjStage::kMeans, means + gb * 3, kProjThreads * 12, &s_bar);
             bulk_load(sm + ProjStage::kScales, scales + gb * 3, kProjThreads * 12, &s_bar);
             bulk_load(sm + ProjStage::kQuats, quats + gb * 4, kProjThreads * 16, &s_bar);
             bulk_load(sm + ProjStage::kOpac, opac + gb, kProjThreads * 4, &s_bar);
-            if (COLORS) bulk_load(sm + ProjStage::kDc, dc + gb * 3, kProjThreads * 12, &s_bar);
+            if (kDc) bulk_load(sm + ProjStage::kDc, dc + gb * 3, kProjThreads * 12, &s_bar);
             if (rs_bytes) bulk_load(sm + ProjStage::kRest, rest + gb * rest_stride, rs_bytes, &s_bar);
             s_fail = !mbar_wait_bounded(&s_bar, 0);
             if (s_fail) {
@@ -153,13 +165,12 @@ project_forward_kernel(const StepParams* __restrict__ P, int N, const float* __r
         for (int e = tid; e < cnt * 3; e += kProjThreads) {
             sm[ProjStage::kMeans + e] = means[gb * 3 + e];
             sm[ProjStage::kScales + e] = scales[gb * 3 + e];
-            if (COLORS) sm[ProjStage::kDc + e] = dc[gb * 3 + e];
+            if (kDc) sm[ProjStage::kDc + e] = dc[gb * 3 + e];
         }
         for (int e = tid; e < cnt * 4; e += kProjThreads) sm[ProjStage::kQuats + e] = quats[gb * 4 + e];
         if (tid < cnt) sm[ProjStage::kOpac + tid] = opac[gb + tid];
-        if (COLORS)
-            for (int e = tid; e < cnt * rest_stride; e += kProjThreads)
-                sm[ProjStage::kRest + e] = rest[gb * rest_stride + e];
+        for (int e = tid; e < cnt * rest_stride; e += kProjThreads)
+            sm[ProjStage::kRest + e] = rest[gb * rest_stride + e];
         __syncthreads();
     }
 
@@ -275,14 +286,37 @@ project_forward_kernel(const StepParams* __restrict__ P, int N, const float* __r
         }
     }
     if (!vis) return;
-    if constexpr (COLORS) {
-        // SH colour (:1780-1786): viewdir = normalize(p - cam_pos)
-        float d0 = p[0] - P->cam_pos[0], d1 = p[1] - P->cam_pos[1], d2 = p[2] - P->cam_pos[2];
-        float dn = rsqrt_ieee((d0 * d0 + d1 * d1) + d2 * d2);
+    // SH colour (:1780-1786): viewdir = normalize(p - cam_pos)
+    float d0 = p[0] - P->cam_pos[0], d1 = p[1] - P->cam_pos[1], d2 = p[2] - P->cam_pos[2];
+    float dn = rsqrt_ieee((d0 * d0 + d1 * d1) + d2 * d2);
+    if constexpr (COLORS == Colors::kFeatures) {
         float col[3];
         float dcv[3] = {s_dc[3 * tid], s_dc[3 * tid + 1], s_dc[3 * tid + 2]};
         sh_to_color(P->degrees_to_use, d0 * dn, d1 * dn, d2 * dn, dcv, s_rest + tid * rest_stride, col);
         out.rgb[i] = make_float4(col[0], col[1], col[2], 0.f);
+    } else {
+        const float d[3] = {d0 * dn, d1 * dn, d2 * dn};
+        const int use = P->degrees_to_use;
+        auto color = [&](auto D) {
+            constexpr int deg = D.value;
+            unsigned w[mx4_words(deg)];
+            if constexpr (COLORS == Colors::kRecords) {
+                mx4_load<deg>(s_rest, tid, w);
+            } else {
+                float q[3 * mx4_rest(deg) + 1];
+#pragma unroll
+                for (int j = 0; j < 3 * mx4_rest(deg); j++) q[j] = s_rest[tid * rest_stride + j];
+                mx4_encode<deg>(s_dc + 3 * tid, q, w);
+            }
+            out.rgb[i] = mx4_view_color<deg>(use, d, w);
+        };
+        // the stride tells the degree: the host checked it
+        constexpr bool kRec = COLORS == Colors::kRecords;
+        if (rest_stride == (kRec ? mx4_words(0) : 0)) color(Degree<0>());
+        else if (rest_stride == (kRec ? mx4_words(1) : 9)) color(Degree<1>());
+        else if (rest_stride == (kRec ? mx4_words(2) : 24)) color(Degree<2>());
+        else if (rest_stride == (kRec ? mx4_words(3) : 45)) color(Degree<3>());
+        else color(Degree<4>());
     }
     if (ZERO_GRADS) {  // training: the SH-rest Adam's copy of the mean
         out.sh_mean[3 * (size_t)i] = p[0];
@@ -313,14 +347,13 @@ void launch_project_forward(const StepParams* P, int N, const float* means, cons
                             const float* quats, const float* dc, const float* rest,
                             const float* opac, const Buffers& B, bool zero_grads,
                             int degrees_to_use_host, int rest_stride_host, cudaStream_t s,
-                            bool colors, bool dropout)
+                            Colors colors, bool dropout)
 {
     (void)degrees_to_use_host;
     if (N <= 0) return;
-    const size_t smem = (size_t)(colors ? ProjStage::kRest + kProjThreads * rest_stride_host
-                                        : ProjStage::kDc) * sizeof(float);
-    uintptr_t mis = (uintptr_t)means | (uintptr_t)scales | (uintptr_t)quats | (uintptr_t)opac;
-    if (colors) mis |= (uintptr_t)dc | (rest_stride_host ? (uintptr_t)rest : 0);
+    const size_t smem = (size_t)(ProjStage::kRest + kProjThreads * rest_stride_host) * sizeof(float);
+    const uintptr_t mis = (uintptr_t)means | (uintptr_t)scales | (uintptr_t)quats |
+                          (uintptr_t)dc | (uintptr_t)opac | (rest_stride_host ? (uintptr_t)rest : 0);
     const int bulk = (mis & 15) == 0 && smem <= 48 * 1024;
     const int grid = (N + kProjThreads - 1) / kProjThreads;
     auto run = [&](auto kernel) {
@@ -328,15 +361,16 @@ void launch_project_forward(const StepParams* P, int N, const float* means, cons
                                                 B.tile_count, zero_grads ? B.grad_acc : nullptr,
                                                 rest_stride_host, bulk, B.err);
     };
-    if (!zero_grads)  // a render: nothing is dropped
-        colors ? run(project_forward_kernel<false, true, false>)
-               : run(project_forward_kernel<false, false, false>);
-    else if (!dropout)
-        colors ? run(project_forward_kernel<true, true, false>)
-               : run(project_forward_kernel<true, false, false>);
+    // a render neither rounds nor drops; a training step has its features
+    if (!zero_grads)
+        colors == Colors::kRecords ? run(project_forward_kernel<false, Colors::kRecords, false>)
+                                   : run(project_forward_kernel<false, Colors::kFeatures, false>);
+    else if (colors == Colors::kRounded)
+        dropout ? run(project_forward_kernel<true, Colors::kRounded, true>)
+                : run(project_forward_kernel<true, Colors::kRounded, false>);
     else
-        colors ? run(project_forward_kernel<true, true, true>)
-               : run(project_forward_kernel<true, false, true>);
+        dropout ? run(project_forward_kernel<true, Colors::kFeatures, true>)
+                : run(project_forward_kernel<true, Colors::kFeatures, false>);
 }
 
 // ---------------------------------------------------------------------------

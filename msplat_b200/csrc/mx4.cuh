@@ -192,7 +192,7 @@ __device__ __forceinline__ void mx4_load(const void* records, long long i,
         const uint4* p = reinterpret_cast<const uint4*>(records) + i * (W / 4);
 #pragma unroll
         for (int k = 0; k < W / 4; k++) {
-            const uint4 v = __ldg(p + k);
+            const uint4 v = p[k];
             w[4 * k] = v.x;
             w[4 * k + 1] = v.y;
             w[4 * k + 2] = v.z;
@@ -202,7 +202,7 @@ __device__ __forceinline__ void mx4_load(const void* records, long long i,
         const uint2* p = reinterpret_cast<const uint2*>(records) + i * (W / 2);
 #pragma unroll
         for (int k = 0; k < W / 2; k++) {
-            const uint2 v = __ldg(p + k);
+            const uint2 v = p[k];
             w[2 * k] = v.x;
             w[2 * k + 1] = v.y;
         }
@@ -291,6 +291,22 @@ __device__ __forceinline__ float mx4_color(int use, const ShDir& D, float dc, fl
                       kSH_C4[8] * (xx * (xx - 3.f * yy) - yy * (3.f * xx - yy)) * r(23));
     }
     return v;
+}
+
+// A record's colour seen along the unit direction d.
+template <int DEG>
+__device__ __forceinline__ float4 mx4_view_color(int use, const float d[3],
+                                                 const unsigned (&w)[mx4_words(DEG)])
+{
+    float dc[3], s[3] = {0.f, 0.f, 0.f}, col[3], q[3 * mx4_rest(DEG) + 1];
+    mx4_dc(w, dc);
+    if constexpr (DEG > 0) mx4_scales(w, s);
+    mx4_codes<DEG>(w, q);
+    const ShDir D = sh_dir(d);
+#pragma unroll
+    for (int c = 0; c < 3; c++)
+        col[c] = mx4_color<DEG>(use, D, dc[c], s[c], [&](int k) { return q[3 * k + c]; });
+    return make_float4(col[0], col[1], col[2], 0.f);
 }
 
 }  // namespace msp

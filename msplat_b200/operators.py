@@ -86,7 +86,7 @@ def dropout(x, rate: float, seed: int, step: int, whole_rows: bool = False, out=
         ys = _rows(out, "out")[2]
     if rows and cols:
         _run("msplat_dropout", x.device, rows, cols, x.data_ptr(), xs, out.data_ptr(), ys, rate,
-             seed & (2**64 - 1), step & (2**64 - 1), int(whole_rows))
+             int(seed) & (2**64 - 1), int(step) & (2**64 - 1), int(bool(whole_rows)))
     return out
 
 

@@ -119,6 +119,8 @@ def test_dropout_values(whole):
     for seed, step in ((5, 7), (4, 6), (5 + 2**32, 6), (5, 6 + 2**32)):
         other = operators.dropout(torch.ones_like(x), 0.5, seed, step, whole_rows=whole) != 0
         assert not torch.equal(other, mask)
+    same = operators.dropout(x, np.float32(0.5), np.int64(-1), np.uint64(6), whole_rows=np.bool_(whole))
+    assert torch.equal(same, operators.dropout(x, 0.5, 2**64 - 1, 6, whole_rows=whole))
     near_one = operators.dropout(x, 1 - 2.0**-31, 5, 6, whole_rows=whole)
     assert bool((near_one == 0).all())
 
@@ -385,6 +387,33 @@ def test_another_stream_and_a_captured_graph():
         if want is want_b:
             want = chain(*b, cams_then, g2)
         assert all(torch.equal(p, q) for p, q in zip(outs, want))
+
+
+def test_calls_at_once():
+    """Threads with streams of their own: each call's result is that of the
+    call alone (nothing is shared between calls)."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    def work(seed):
+        dc, rest = oc.features(20_000 + seed, 3, seed)
+        _, means, cams, _ = case(20_000 + seed, 3, 2, seed)
+        x, g = dev(rest.reshape(len(rest), 45)), torch.ones(2, len(rest), 3, device="cuda")
+        return [x, dev(dc), dev(rest), dev(means)], cams, g
+    inputs = [work(s) for s in range(4)]
+    want = [chain(*a, cams, g) for a, cams, g in inputs]
+    torch.cuda.synchronize()
+
+    def run(k):
+        a, cams, g = inputs[k]
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                out = chain(*a, cams, g)
+        stream.synchronize()
+        return out
+    with ThreadPoolExecutor(4) as pool:
+        for got, w in zip(pool.map(run, range(4)), want):
+            assert all(torch.equal(p, q) for p, q in zip(got, w))
 
 
 def test_python_refusals_on_tensors():

@@ -140,7 +140,8 @@ def test_render_mx4_leaves_other_renders_alone():
 # ---- training with 4-bit colours
 
 @pytest.mark.parametrize("n, w, h, degree, use", [(8_000, 200, 160, 3, 3), (8_001, 480, 330, 3, 1),
-                                                  (5_000, 480, 330, 2, 2), (5_000, 480, 330, 0, 0)])
+                                                  (5_000, 480, 330, 2, 2), (5_000, 480, 330, 0, 0),
+                                                  (5_003, 480, 330, 1, 1), (3_000, 480, 330, 4, 4)])
 def test_step_with_mx4_colors(n, w, h, degree, use):
     import torch
     g, cs = scene(n, w, h, seed=7, degree=degree, use=use)
