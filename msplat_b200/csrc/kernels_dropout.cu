@@ -5,6 +5,7 @@
 // rounds of two wide multiplications and two three-way exclusive ors) serves
 // four draws.
 #include <algorithm>
+#include <type_traits>
 
 #include "dropout.cuh"
 #include "engine.h"
@@ -25,35 +26,7 @@ struct DropArgs {
     PhiloxKeys keys;
 };
 
-// One draw per element, arrays without gaps at 16-byte alignment.  A thread
-// takes the four elements of one Philox group as one vector.  40M elements:
-// 54 us (5.9 TB/s).
-__global__ void __launch_bounds__(kDropThreads)
-dropout_vector_kernel(DropArgs a, long long total)
-{
-    const long long groups = (total + 3) >> 2;
-    for (long long g = blockIdx.x * (long long)kDropThreads + threadIdx.x; g < groups;
-         g += (long long)gridDim.x * kDropThreads) {
-        const long long i0 = g << 2;
-        const bool whole = i0 + 4 <= total;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (whole) v = *reinterpret_cast<const float4*>(a.x + i0);   // in flight under the draws
-        const uint4 d = philox4x32((unsigned long long)g, a.step, a.keys);
-        if (whole) {
-            v.x = d.x >= a.threshold ? v.x * a.scale : 0.f;
-            v.y = d.y >= a.threshold ? v.y * a.scale : 0.f;
-            v.z = d.z >= a.threshold ? v.z * a.scale : 0.f;
-            v.w = d.w >= a.threshold ? v.w * a.scale : 0.f;
-            *reinterpret_cast<float4*>(a.y + i0) = v;
-        } else {
-            const unsigned u[4] = {d.x, d.y, d.z, d.w};
-            for (int k = 0; i0 + k < total; k++)
-                a.y[i0 + k] = u[k] >= a.threshold ? a.x[i0 + k] * a.scale : 0.f;
-        }
-    }
-}
-
-// The other kernels give a block a chunk of consecutive elements: one 64-bit
+// A block takes a chunk of consecutive elements: one 64-bit
 // division finds the chunk's first row, and an element's row and column in
 // the chunk come from 32-bit arithmetic.  (Dividing each element's 64-bit
 // index took 34 us a pass over 333,337 rows of 23, of which the traffic is 10.)
@@ -61,8 +34,11 @@ constexpr int kChunkElems = 8192;
 
 // Row of place t = (column of the chunk's first element) + (element of the
 // chunk), counted from the chunk's first row.  Exact: t < cols + 8192 and, by
-// `magic` = ceil(2^32 / cols) for 2 <= cols <= 8192, t * cols < 2^32.
-enum RowRule { kOneColumn, kByMagic, kWideRows };
+// `magic` = ceil(2^32 / cols) for 2 <= cols <= 8192, t * cols < 2^32.  kNoGaps:
+// an element's index is its place, and no row is needed.
+enum RowRule { kOneColumn, kByMagic, kWideRows, kNoGaps };
+template <RowRule RULE>
+using Rule = std::integral_constant<RowRule, RULE>;
 template <RowRule RULE>
 __device__ __forceinline__ int local_row(unsigned t, int cols, unsigned magic)
 {
@@ -74,33 +50,44 @@ __device__ __forceinline__ int local_row(unsigned t, int cols, unsigned magic)
 // elements; each lane draws two groups' four, and ballots turn the draws into
 // a bit per element, so that every access is of 32 neighbours and not of each
 // lane's own four.  Offset: the type that holds a row offset in a chunk (32
-// bits for all but the widest strides).  Bound by instructions, the draws'
-// and the indexes': 333,337 rows of 23 in rows of 27, 16.5 us a pass (3.7
-// TB/s); 40M elements off alignment 83 us.  48 registers (5 blocks a
-// multiprocessor) 18.1 us, 78 without that bound 21.4.  `magic64` = ceil(2^64 / cols) divides the chunk's first
+// bits for all but the widest strides); YGAPS: y's rows are apart.  40M
+// elements without gaps: 54 us (5.9 TB/s), at any alignment -- a vector an access
+// is no faster.  With gaps it is bound by instructions, the draws' and the
+// indexes': 333,337 rows of 23 in rows of 27, 15.2 us a pass (4.0 TB/s).  48
+// registers: 18.1 us where 78 took 21.4.
+// `magic64` = ceil(2^64 / cols) divides the chunk's first
 // index exactly while index * cols < 2^64; 0: plain division.
 constexpr int kElemsChunk = 256 * (kDropThreads / 32);
 
-template <RowRule RULE, typename Offset, bool FULL>
+template <RowRule RULE, typename Offset, bool YGAPS, bool FULL>
 __device__ __forceinline__ void dropout_chunk(const DropArgs& a, long long i0, int cnt,
                                               unsigned magic, unsigned long long magic64)
 {
     const int lane = threadIdx.x & 31;
     const int e0 = 256 * (threadIdx.x >> 5) + lane;
-    const long long r0 = magic64 ? (long long)__umul64hi((unsigned long long)i0, magic64) : i0 / a.cols;
-    const unsigned c0 = (unsigned)(i0 - r0 * a.cols);
-    const float* x = a.x + r0 * a.x_stride;
-    float* y = a.y + r0 * a.y_stride;
+    long long r0 = 0;
+    unsigned c0 = 0;
+    if (RULE != kNoGaps) {
+        r0 = magic64 ? (long long)__umul64hi((unsigned long long)i0, magic64) : i0 / a.cols;
+        c0 = (unsigned)(i0 - r0 * a.cols);
+    }
+    const float* x = RULE == kNoGaps ? a.x + i0 + e0 : a.x + r0 * a.x_stride;
+    float* y = YGAPS ? a.y + r0 * a.y_stride : a.y + i0 + e0;
     float v[8];
     Offset to[8];
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-        const unsigned t = c0 + e0 + 32 * k;
-        const int r = local_row<RULE>(t, a.cols, magic);
-        const int c = (int)(t - (unsigned)r * (unsigned)a.cols);
-        to[k] = (Offset)r * (Offset)a.y_stride + c;
+        Offset from = 32 * k;
+        to[k] = 32 * k;
+        if (RULE != kNoGaps) {
+            const unsigned t = c0 + e0 + 32 * k;
+            const int r = local_row<RULE>(t, a.cols, magic);
+            const int c = (int)(t - (unsigned)r * (unsigned)a.cols);
+            from = (Offset)r * (Offset)a.x_stride + c;
+            if (YGAPS) to[k] = (Offset)r * (Offset)a.y_stride + c;
+        }
         v[k] = 0.f;
-        if (FULL || e0 + 32 * k < cnt) v[k] = x[(Offset)r * (Offset)a.x_stride + c];   // in flight under the draws
+        if (FULL || e0 + 32 * k < cnt) v[k] = x[from];   // in flight under the draws
     }
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -119,7 +106,7 @@ __device__ __forceinline__ void dropout_chunk(const DropArgs& a, long long i0, i
     }
 }
 
-template <RowRule RULE, typename Offset>
+template <RowRule RULE, typename Offset, bool YGAPS>
 __global__ void __launch_bounds__(kDropThreads, 5)
 dropout_elements_kernel(DropArgs a, long long total, unsigned magic, unsigned long long magic64)
 {
@@ -127,9 +114,9 @@ dropout_elements_kernel(DropArgs a, long long total, unsigned magic, unsigned lo
     for (long long ch = blockIdx.x; ch < chunks; ch += gridDim.x) {
         const long long i0 = ch * kElemsChunk;
         if (i0 + kElemsChunk <= total)
-            dropout_chunk<RULE, Offset, true>(a, i0, kElemsChunk, magic, magic64);
+            dropout_chunk<RULE, Offset, YGAPS, true>(a, i0, kElemsChunk, magic, magic64);
         else
-            dropout_chunk<RULE, Offset, false>(a, i0, (int)(total - i0), magic, magic64);
+            dropout_chunk<RULE, Offset, YGAPS, false>(a, i0, (int)(total - i0), magic, magic64);
     }
 }
 
@@ -140,7 +127,10 @@ dropout_elements_kernel(DropArgs a, long long total, unsigned magic, unsigned lo
 // access starts at one).  1M rows of 45 at rate 0.2, both directions: 106 us
 // (6.8 TB/s of the bytes of all rows; the dropped fifth is not read), against
 // 292 with an element an access.
-template <RowRule RULE, bool VEC>
+// Otherwise eight accesses of an element each are under way at once; XGAPS and
+// YGAPS say whose rows are apart, Offset as above.  800,000 rows of 45 off
+// alignment: 54 us (5.4 TB/s), aligned 46.
+template <RowRule RULE, bool VEC, typename Offset, bool XGAPS, bool YGAPS>
 __global__ void __launch_bounds__(kDropThreads)
 dropout_rows_kernel(DropArgs a, long long total, unsigned magic)
 {
@@ -206,16 +196,26 @@ dropout_rows_kernel(DropArgs a, long long total, unsigned magic)
             }
             continue;
         }
-        const float* x = a.x + r0 * a.x_stride;
-        float* y = a.y + r0 * a.y_stride;
-#pragma unroll 4
-        for (int e = threadIdx.x; e < cnt; e += kDropThreads) {
-            const unsigned t = c0 + e;
-            const int r = local_row<RULE>(t, a.cols, magic);
-            const int c = (int)(t - (unsigned)r * (unsigned)a.cols);
-            const float f = scale[r];
-            const float v = f != 0.f ? x[r * a.x_stride + c] : 0.f;
-            y[r * a.y_stride + c] = v * f;
+        const float* x = XGAPS ? a.x + r0 * a.x_stride : a.x + i0;
+        float* y = YGAPS ? a.y + r0 * a.y_stride : a.y + i0;
+        constexpr int kU = 8;
+        for (int e0 = threadIdx.x; e0 < cnt; e0 += kDropThreads * kU) {
+            float v[kU], f[kU];
+            Offset to[kU];
+#pragma unroll
+            for (int u = 0; u < kU; u++) {
+                const int e = e0 + u * kDropThreads;
+                const unsigned t = c0 + e;
+                const int r = local_row<RULE>(t, a.cols, magic);
+                const int c = (int)(t - (unsigned)r * (unsigned)a.cols);
+                to[u] = YGAPS ? (Offset)r * (Offset)a.y_stride + c : (Offset)e;
+                f[u] = e < cnt ? scale[r] : 0.f;
+                v[u] = 0.f;   // a dropped value may be anything, a NaN too: no product
+                if (f[u] != 0.f) v[u] = x[XGAPS ? (Offset)r * (Offset)a.x_stride + c : (Offset)e];
+            }
+#pragma unroll
+            for (int u = 0; u < kU; u++)
+                if (e0 + u * kDropThreads < cnt) y[to[u]] = v[u] * f[u];
         }
     }
 }
@@ -251,44 +251,51 @@ extern "C" int msplat_dropout(long long rows, int cols, const float* x, long lon
     const DropArgs a{x, y, rows, x_stride, y_stride, cols, dr.threshold, dr.scale, step, philox_keys(seed)};
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     const long long total = rows * cols;
-    const bool flat = x_stride == cols && y_stride == cols;
+    const bool xgaps = x_stride != cols, ygaps = y_stride != cols, flat = !xgaps && !ygaps;
     const bool aligned = flat && (((uintptr_t)x | (uintptr_t)y) & 15) == 0;
-    auto blocks = [](long long items, long long per) {
-        return (unsigned)std::min<long long>((items + per - 1) / per, 1 << 20);
-    };
     const unsigned magic =
         cols >= 2 && cols <= kChunkElems ? (unsigned)(((1ULL << 32) + cols - 1) / cols) : 0u;
+    auto blocks = [&](long long per) {
+        return (unsigned)std::min<long long>((total + per - 1) / per, 1 << 20);
+    };
+    // whether a row offset within a chunk fits 32 bits
+    auto narrow = [&](long long per) {
+        return (per / cols + 2) * std::max(x_stride, y_stride) < 1LL << 31;
+    };
     if (whole_rows && cols > 1) {
         auto run = [&](auto kernel) {
-            kernel<<<blocks(total, kChunkElems), kDropThreads, 0, st>>>(a, total, magic);
+            kernel<<<blocks(kChunkElems), kDropThreads, 0, st>>>(a, total, magic);
         };
-        if (aligned)
-            magic ? run(dropout_rows_kernel<kByMagic, true>) : run(dropout_rows_kernel<kWideRows, true>);
-        else
-            magic ? run(dropout_rows_kernel<kByMagic, false>) : run(dropout_rows_kernel<kWideRows, false>);
-    } else if (aligned) {
-        dropout_vector_kernel<<<blocks(total, 4 * kDropThreads), kDropThreads, 0, st>>>(a, total);
+        auto pick = [&](auto R) {
+            constexpr RowRule rule = R.value;
+            if (aligned) run(dropout_rows_kernel<rule, true, int, false, false>);
+            else if (flat) run(dropout_rows_kernel<rule, false, int, false, false>);
+            else if (narrow(kChunkElems))
+                ygaps ? run(dropout_rows_kernel<rule, false, int, true, true>)
+                      : run(dropout_rows_kernel<rule, false, int, true, false>);
+            else
+                ygaps ? run(dropout_rows_kernel<rule, false, long long, true, true>)
+                      : run(dropout_rows_kernel<rule, false, long long, true, false>);
+        };
+        magic ? pick(Rule<kByMagic>()) : pick(Rule<kWideRows>());
     } else {
-        DropArgs e = a;
-        if (flat) {  // one long row: an element's index is its place
-            e.cols = 1 << 29;
-            e.x_stride = e.y_stride = e.cols;
-        }
-        const bool fits = e.cols > 1 && total < (1LL << 62) / e.cols;
-        const unsigned long long magic64 = fits ? ~0ULL / (unsigned)e.cols + 1 : 0;
-        const bool narrow = (kElemsChunk / e.cols + 2) * std::max(e.x_stride, e.y_stride) < 1LL << 31;
+        const bool fits = cols > 1 && total < (1LL << 62) / cols;
+        const unsigned long long magic64 = fits ? ~0ULL / (unsigned)cols + 1 : 0;
         auto run = [&](auto kernel) {
-            kernel<<<blocks(total, kElemsChunk), kDropThreads, 0, st>>>(e, total, magic, magic64);
+            kernel<<<blocks(kElemsChunk), kDropThreads, 0, st>>>(a, total, magic, magic64);
         };
-        if (e.cols == 1)
-            narrow ? run(dropout_elements_kernel<kOneColumn, int>)
-                   : run(dropout_elements_kernel<kOneColumn, long long>);
-        else if (e.cols <= kChunkElems)
-            narrow ? run(dropout_elements_kernel<kByMagic, int>)
-                   : run(dropout_elements_kernel<kByMagic, long long>);
-        else
-            narrow ? run(dropout_elements_kernel<kWideRows, int>)
-                   : run(dropout_elements_kernel<kWideRows, long long>);
+        auto pick = [&](auto R) {
+            constexpr RowRule rule = R.value;
+            if (narrow(kElemsChunk))
+                ygaps ? run(dropout_elements_kernel<rule, int, true>)
+                      : run(dropout_elements_kernel<rule, int, false>);
+            else
+                ygaps ? run(dropout_elements_kernel<rule, long long, true>)
+                      : run(dropout_elements_kernel<rule, long long, false>);
+        };
+        if (flat) run(dropout_elements_kernel<kNoGaps, int, false>);
+        else if (cols == 1) pick(Rule<kOneColumn>());
+        else magic ? pick(Rule<kByMagic>()) : pick(Rule<kWideRows>());
     }
     return launched("msplat_dropout", 1);
 }
