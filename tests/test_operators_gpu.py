@@ -47,7 +47,8 @@ def check_dropout(got, x, rate, seed, step, whole):
 @pytest.mark.parametrize("whole", [False, True])
 @pytest.mark.parametrize("rows, cols", [(1, 1), (2, 1), (3, 1), (5, 1), (1023, 1), (4096, 1), (1, 45),
                                         (127, 45), (128, 45), (129, 45), (1000, 3), (257, 24),
-                                        (33, 129), (3, 6001), (1001, 2)])
+                                        (33, 129), (3, 6001), (1001, 2), (2, 8192), (5, 9001),
+                                        (1, 50_000)])
 def test_dropout(rows, cols, whole):
     rng = np.random.default_rng(rows * 1000 + cols)
     x = rng.normal(size=(rows, cols)).astype(np.float32)
@@ -58,10 +59,10 @@ def test_dropout(rows, cols, whole):
 
 @pytest.mark.parametrize("whole", [False, True])
 @pytest.mark.parametrize("off, pad", [(0, 4), (1, 3), (2, 0), (3, 1)])
-def test_dropout_layouts(off, pad, whole):
+@pytest.mark.parametrize("rows, cols", [(301, 20), (5000, 1), (3000, 2), (7, 9001)])
+def test_dropout_layouts(rows, cols, off, pad, whole):
     """Rows inside a wider array, at any alignment: the result is that of the
     same values side by side, and nothing outside the rows is written."""
-    rows, cols = 301, 20
     rng = np.random.default_rng(off * 10 + pad)
     base = dev(rng.normal(size=(rows * (cols + pad) + 8,)).astype(np.float32))
     x = base[off:off + rows * (cols + pad)].view(rows, cols + pad)[:, :cols]
@@ -134,13 +135,18 @@ def test_dropout_past_32_bits():
     del x
     kept, _ = oc.keep(np.arange(n - 128, n), 0.5, 9, 8)
     np.testing.assert_array_equal(tail, np.where(kept, 2.0, 0.0))
-    rows, stride = 70_000, 62_001
-    wide = torch.empty(rows * stride, device="cuda").view(rows, stride)
-    for cols, whole in ((2, False), (2, True)):
-        wide[:, :cols] = 1
-        out = operators.dropout(wide[:, :cols], 0.5, 8, 9, whole_rows=whole)
-        check_dropout(host(out), np.ones((rows, cols), np.float32), 0.5, 8, 9, whole)
-    del wide
+    # the last two: rows so far apart that offsets within a block's share pass it
+    for rows, stride, widths in ((70_000, 62_001, (2, 1)), (1100, 2_100_001, (2, 1, 45)),
+                                 (3, 1_100_000_001, (9001,))):
+        wide = torch.empty(rows * stride, device="cuda").view(rows, stride)
+        for cols in widths:
+            for whole in (False, True):
+                x = wide[:, :cols]
+                x.fill_(1)
+                out = operators.dropout(x, 0.5, 8, 9, whole_rows=whole)
+                check_dropout(host(out), np.ones((rows, cols), np.float32), 0.5, 8, 9, whole)
+                assert torch.equal(operators.dropout(x, 0.5, 8, 9, whole_rows=whole, out=x), out)
+        del wide, x
     torch.cuda.empty_cache()
 
 
