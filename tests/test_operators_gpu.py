@@ -188,7 +188,8 @@ def test_pack_awkward_values(degree):
     rec = operators.mx4_pack(dev(dc), dev(rest))
     want = oc.encode(dc, rest)
     # a NaN has many bit patterns
-    nan = np.isnan(dc.astype(np.float16))
+    with np.errstate(over="ignore"):
+        nan = np.isnan(dc.astype(np.float16))
     got = host(rec)
     gdc, grest = operators.mx4_unpack(rec, degree)
     np.testing.assert_array_equal(np.isnan(host(gdc)), nan)
@@ -286,6 +287,52 @@ def test_colors_special_rows():
     out = torch.full((2, 50, 3), 7.0, device="cuda")
     operators.mx4_colors(dev(rec), 3, dev(means), cams, radii=dev(np.zeros((2, 50), np.int32)), out=out)
     assert bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("n", [1, 33, 128, 300])
+@pytest.mark.parametrize("off", [0, 1, 4])
+def test_nothing_outside_the_outputs_is_written(n, off):
+    """Colours, their gradients and unpacked features into the middle of larger
+    arrays, at any alignment: the same values, and the floats around stay."""
+    for degree, views in ((0, 1), (1, 2), (2, 1), (3, 1), (3, 3), (4, 1)):
+        rec, means, cams, radii = case(n, degree, views, seed=off + n)
+        g = torch.randn(views, n, 3, device="cuda")
+
+        def room(*shape):
+            size = int(np.prod(shape))
+            t = torch.full((size + 12,), 7.0, device="cuda")
+            return t, t[off + 4:off + 4 + size].view(shape)
+
+        def around(t, view):
+            t = t.clone()
+            t[off + 4:off + 4 + view.numel()] = 7.0
+            assert bool((t == 7.0).all())
+        for r in (None, dev(radii)):
+            whole, out = room(views, n, 3)
+            out.zero_()
+            operators.mx4_colors(dev(rec), degree, dev(means), cams, radii=r, out=out)
+            assert torch.equal(out, operators.mx4_colors(dev(rec), degree, dev(means), cams, radii=r))
+            around(whole, out)
+            (w0, o0), (w1, o1) = room(n, 3), room(n, oc.REST[degree], 3)
+            operators.mx4_colors_backward(g, degree, dev(means), cams, radii=r, out=(o0, o1))
+            want = operators.mx4_colors_backward(g, degree, dev(means), cams, radii=r)
+            assert torch.equal(o0, want[0]) and torch.equal(o1, want[1])
+            around(w0, o0)
+            around(w1, o1)
+        operators.mx4_unpack(dev(rec), degree, out=(o0, o1))
+        want = operators.mx4_unpack(dev(rec), degree)
+        assert torch.equal(o0, want[0]) and torch.equal(o1, want[1])
+        around(w0, o0)
+        around(w1, o1)
+
+
+def test_one_view_is_a_row_of_several():
+    """The variants for one view and for several give the same bits."""
+    rec, means, cams, radii = case(5000, 3, 4, seed=77)
+    many = operators.mx4_colors(dev(rec), 3, dev(means), cams)
+    for v in range(4):
+        one = operators.mx4_colors(dev(rec), 3, dev(means), cams[v:v + 1])
+        assert torch.equal(one[0], many[v])
 
 
 def test_colors_past_32_bits():

@@ -289,6 +289,30 @@ def test_dropped_gaussians_are_culled_ones_to_adam():
     assert vis.any() and (model.params[3].cpu().numpy()[vis] != g.features_dc[vis]).any(1).mean() > 0.9
 
 
+@pytest.mark.parametrize("w, h", [(200, 160), (480, 330)])
+def test_step_in_which_everything_is_dropped(w, h):
+    """The background, no gradient, moments that decay from zero: a step like
+    any other, and the next one is too."""
+    import torch
+    g, cs = scene(2_000, w, h, seed=14)
+    gt = torch.as_tensor(synthetic.target_image(w, h, 1)).cuda()
+    model = engine.GaussianModel(g.groups())
+    engine.set_step_options(dropout_rate=1 - 2.0**-31, dropout_seed=1, dropout_step=1, mx4_colors=True)
+    got, vis = grads(g, cs, gt)
+    assert not vis.any() and not any(p.any() for p in got)
+    img = engine.debug_buffer("out_img", 3 * w * h, np.float32).reshape(h, w, 3)
+    np.testing.assert_array_equal(img, np.broadcast_to(np.float32(engine.DEFAULT_BG), img.shape))
+    engine.train_step(model, cs, gt)
+    for k in range(6):
+        np.testing.assert_array_equal(model.params[k].cpu().numpy(), g.groups()[k])
+    assert _lib.load().msplat_device_errors() == 0
+    engine.set_step_options()
+    engine.render(engine.GaussianModel(g.groups()), cs)
+    want = dump(cs, g.n)
+    engine.render(model, cs)
+    np.testing.assert_array_equal(dump(cs, g.n)["out_img"], want["out_img"])
+
+
 def test_views_of_one_step_share_the_mask():
     import torch
     g, _ = scene(2_000, 320, 240, seed=8)
