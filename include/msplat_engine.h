@@ -618,7 +618,8 @@ int msplat_mx4_unpack(int n, int degree, const void *records, float *features_dc
  * (it adds 0.5 and clamps at 0); the sums are fused multiply-adds, so its last
  * bits are not the renderer's.  With radii (num_views,n; NULL: all visible) the
  * colours of Gaussians of radius <= 0 are not written.  A mean at the camera
- * has no direction: its colour is NaN unless degrees_to_use is 0. */
+ * has no direction: its colour, and the gradient below, is NaN unless
+ * degrees_to_use is 0.  Distances from 1e-18 to 1e18. */
 int msplat_mx4_colors(int n, int degree, int degrees_to_use, const float *means3d,
                       const void *records, int num_views, const float *cam_pos,
                       const int32_t *radii, float *colors, void *cuda_stream);

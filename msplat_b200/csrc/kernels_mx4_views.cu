@@ -1,7 +1,8 @@
 // kernels_mx4_views.cu -- the colours of a batch of views from 4-bit records
 // (format in mx4.cuh) and the gradient of the coefficients.  Compiled with FMA
 // contraction: a fused multiply-add per coefficient and view is what bounds
-// many views.  (A renderer's view, kernels_mx4.cu, keeps the projection's bits.)
+// many views.  (A rendered view's colours come from the projection, kernels_fwd.cu,
+// and have its bits.)
 #include <algorithm>
 
 #include "mx4_rows.cuh"
