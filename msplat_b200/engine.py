@@ -347,8 +347,9 @@ class PackedGaussians:
         stream (bind_stream() makes it the engine's)."""
         from . import operators
         p = model.params
-        return cls(p[0].clone(), p[1].clone(), p[2].clone(), p[5].clone(),
-                   operators.mx4_pack(p[3], p[4]), model.sh_degree)
+        records = operators.mx4_pack(p[3], p[4])
+        degree = operators.REST_BASES.index(model.rest_bases)   # a record's, whatever is in use
+        return cls(p[0].clone(), p[1].clone(), p[2].clone(), p[5].clone(), records, degree)
 
     @property
     def n(self) -> int:
