@@ -163,6 +163,15 @@ def test_python_refusals():
 
 # ---- options of the training step and the packed renderer
 
+def test_packed_scene_refusals():
+    from msplat_b200 import engine
+    t = torch.zeros
+    with pytest.raises(ValueError, match="degree"):
+        engine.PackedGaussians(t(4, 3), t(4, 3), t(4, 4), t(4, 1), t(4, 32, dtype=torch.uint8), 7)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        engine.PackedGaussians(t(4, 3), t(4, 3), t(4, 4), t(4, 1), t(4, 32, dtype=torch.uint8), 3)
+
+
 def test_option_refusals(lib):
     for rate in (-0.5, 1.0, float("nan")):
         refused(lib, lib.msplat_set_step_options(C.byref(_lib.MsplatStepOptions(rate, 1, 2, 0))),

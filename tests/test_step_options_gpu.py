@@ -385,6 +385,21 @@ def test_dropout_opacity_gradient_against_differences():
 
 # ---- refusals, and options together in the trainer
 
+def test_packed_scene_refuses_what_does_not_fit():
+    """A scene whose arrays disagree would be read out of range."""
+    import torch
+    g, _ = scene(100, 64, 48, seed=1)
+    p = engine.PackedGaussians.of(engine.GaussianModel(g.groups()))
+    parts = dict(means=p.means, scales=p.scales, quats=p.quats, opacities=p.opacities, records=p.records,
+                 sh_degree=3)
+    engine.PackedGaussians(**parts)
+    for name, bad in (("means", p.means[:99]), ("scales", p.scales.double()), ("quats", p.quats[:, :3]),
+                      ("opacities", p.opacities[:, 0]), ("records", p.records[:99]), ("sh_degree", 2),
+                      ("means", p.means.cpu()), ("quats", torch.zeros(4, 100, device="cuda").t())):
+        with pytest.raises(ValueError):
+            engine.PackedGaussians(**dict(parts, **{name: bad}))
+
+
 def test_step_refuses_wrong_bases():
     import torch
     g, cs = scene(500, 64, 48, seed=1, degree=2)
