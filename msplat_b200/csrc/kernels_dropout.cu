@@ -26,10 +26,10 @@ struct DropArgs {
     PhiloxKeys keys;
 };
 
-// A block takes a chunk of consecutive elements: one 64-bit
-// division finds the chunk's first row, and an element's row and column in
-// the chunk come from 32-bit arithmetic.  (Dividing each element's 64-bit
-// index took 34 us a pass over 333,337 rows of 23, of which the traffic is 10.)
+// A block takes a chunk of consecutive elements: one 64-bit division finds the
+// chunk's first row, and an element's row and column in the chunk come from
+// 32-bit arithmetic.  (Dividing each element's 64-bit index took 34 us a pass
+// over 333,337 rows of 23, of which the traffic is 10.)
 constexpr int kChunkElems = 8192;
 
 // Row of place t = (column of the chunk's first element) + (element of the
@@ -55,8 +55,8 @@ __device__ __forceinline__ int local_row(unsigned t, int cols, unsigned magic)
 // is no faster.  With gaps it is bound by instructions, the draws' and the
 // indexes': 333,337 rows of 23 in rows of 27, 15.2 us a pass (4.0 TB/s).  48
 // registers: 18.1 us where 78 took 21.4.
-// `magic64` = ceil(2^64 / cols) divides the chunk's first
-// index exactly while index * cols < 2^64; 0: plain division.
+// `magic64` = ceil(2^64 / cols) divides the chunk's first index exactly while
+// index * cols < 2^64; 0: plain division.
 constexpr int kElemsChunk = 256 * (kDropThreads / 32);
 
 template <RowRule RULE, typename Offset, bool YGAPS, bool FULL>

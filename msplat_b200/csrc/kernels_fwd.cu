@@ -110,7 +110,8 @@ struct ProjStage {
 // step).  kRecords stages records instead of dc and rows: 76 of 236 bytes a
 // Gaussian at degree 3, a render of 6M in 1.50 ms (1.59 from features), of 1M in
 // 0.596 (0.615); by a kernel of their own on another stream, beside binning and
-// sorting, the colours took 1.52 and 0.587.  With DROPOUT a Gaussian that its draw drops is culled -- not binned, sorted,
+// sorting, the colours took 1.52 and 0.587.
+// With DROPOUT a Gaussian that its draw drops is culled -- not binned, sorted,
 // blended nor given gradients -- and the others' opacity is multiplied by
 // drop_scale.
 template <bool ZERO_GRADS, Colors COLORS, bool DROPOUT>
