@@ -307,7 +307,9 @@ raster_backward_kernel(const StepParams* __restrict__ P, const int* __restrict__
                     if (j >= 3 && j < 6) x *= 0.5f;
                     if (ok) atomicAdd(grad_acc + (size_t)g * kGradStride + j, x);
                 } else if (lane == 1) {
-                    if (vop != 0.f) atomicAdd(grad_acc + (size_t)g * kGradStride + 8, -(1.f - (DROPOUT ? co.w * P->drop_inv : co.w)) * vop);
+                    if (vop != 0.f)
+                        atomicAdd(grad_acc + (size_t)g * kGradStride + 8,
+                                  -(1.f - (DROPOUT ? co.w * P->drop_inv : co.w)) * vop);
                 }
             }
         }
