@@ -150,13 +150,13 @@ def mx4_unpack(records, degree: int, out=None):
 
 
 def _views(cam_pos):
-    """Camera positions as a C-ordered float32 array (V, 3) on the host."""
+    """Camera positions as C-ordered float32 (V, 3) in host bytes, and V."""
     if isinstance(cam_pos, torch.Tensor):
         raise ValueError("cam_pos is host data: an array or nested list of shape (V, 3)")
     cams = np.ascontiguousarray(cam_pos, dtype=np.float32)
     if cams.ndim != 2 or cams.shape[1] != 3 or cams.shape[0] > MAX_VIEWS:
         raise ValueError(f"cam_pos must have shape (V, 3), V <= {MAX_VIEWS}, not {cams.shape}")
-    return cams, cams.shape[0]
+    return cams.tobytes(), cams.shape[0]
 
 
 def _use(degrees_to_use, degree: int) -> int:
@@ -188,7 +188,7 @@ def mx4_colors(records, degree: int, means, cam_pos, degrees_to_use=None, radii=
     else:
         _check(out, "out", (views, n, 3), device=dev)
     _run("msplat_mx4_colors", dev, n, degree, use, means.data_ptr(), records.data_ptr(), views,
-         cams.ctypes.data, rp, out.data_ptr())
+         cams, rp, out.data_ptr())
     return out
 
 
@@ -208,10 +208,10 @@ def mx4_colors_backward(v_colors, degree: int, means, cam_pos, degrees_to_use=No
     rp = _radii(radii, views, n, dev)
     shapes = ((n, 3), (n, REST_BASES[degree], 3))
     if out is None:
-        out = tuple(means.new_empty(s) for s in shapes)
+        out = (torch.empty_like(means), means.new_empty(shapes[1]))
     else:
         for t, s, name in zip(out, shapes, ("out[0]", "out[1]"), strict=True):
             _check(t, name, s, device=dev)
     _run("msplat_mx4_colors_backward", dev, n, degree, use, means.data_ptr(), views,
-         cams.ctypes.data, rp, v_colors.data_ptr(), out[0].data_ptr(), out[1].data_ptr())
+         cams, rp, v_colors.data_ptr(), out[0].data_ptr(), out[1].data_ptr())
     return out
