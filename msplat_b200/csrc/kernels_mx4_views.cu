@@ -181,8 +181,7 @@ constexpr int one_view_blocks(int deg) { return deg == 4 ? 6 : 8; }
 template <int DEG, int USE, bool MASKED>
 __global__ void __launch_bounds__(kMxThreads, one_view_blocks(DEG))
 mx4_colors_one_kernel(int n, const float* __restrict__ means, const void* __restrict__ records,
-                      int, const Mx4Cams cams, const int* __restrict__ radii,
-                      float* __restrict__ colors)
+                      const Mx4Cam cam, const int* __restrict__ radii, float* __restrict__ colors)
 {
     __shared__ float s_col[kMxThreads * 3];
     const long long step = (long long)gridDim.x * kMxThreads;
@@ -195,7 +194,7 @@ mx4_colors_one_kernel(int n, const float* __restrict__ means, const void* __rest
         const bool on_after = visible(i + 2 * step);
         if (on_next) g_next.load(means, records, i + step);
         float col[3];
-        color_of_record<DEG, USE>(cams.p[0], g, col);
+        color_of_record<DEG, USE>(cam.p, g, col);
         const long long i0 = i - (threadIdx.x & 31);
         const unsigned mask = MASKED ? __ballot_sync(0xffffffffu, on) : 0u;
         put_colors<!MASKED>(colors + 3 * i0, s_col, col, mask, floats_left(n, i0));
@@ -348,16 +347,18 @@ int msplat_mx4_colors(int n, int degree, int degrees_to_use, const float* means3
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     with_degrees(degree, degrees_to_use, [&](auto D, auto U) {
         constexpr int d = D.value, u = U.value;
-        auto run = [&](auto kernel, unsigned blocks) {
-            kernel<<<blocks, kMxThreads, 0, st>>>(n, means3d, records, num_views, cams, radii, colors);
-        };
         const unsigned tiles = mx4_blocks(n), stay = std::min(tiles, 148u * one_view_blocks(d));
+        auto one = [&](auto kernel) {
+            const Mx4Cam cam = {{cam_pos[0], cam_pos[1], cam_pos[2]}};
+            kernel<<<stay, kMxThreads, 0, st>>>(n, means3d, records, cam, radii, colors);
+        };
+        auto several = [&](auto kernel) {
+            kernel<<<tiles, kMxThreads, 0, st>>>(n, means3d, records, num_views, cams, radii, colors);
+        };
         if (num_views == 1)
-            radii ? run(mx4_colors_one_kernel<d, u, true>, stay)
-                  : run(mx4_colors_one_kernel<d, u, false>, stay);
+            radii ? one(mx4_colors_one_kernel<d, u, true>) : one(mx4_colors_one_kernel<d, u, false>);
         else
-            radii ? run(mx4_colors_kernel<d, u, true>, tiles)
-                  : run(mx4_colors_kernel<d, u, false>, tiles);
+            radii ? several(mx4_colors_kernel<d, u, true>) : several(mx4_colors_kernel<d, u, false>);
     });
     return launched(who, 1);
 }

@@ -42,6 +42,9 @@ __host__ __device__ constexpr int mx4_align(int degree) { return degree == 0 || 
 struct Mx4Cams {
     float p[kMx4MaxViews][3];
 };
+struct Mx4Cam {
+    float p[3];
+};
 
 // Eight floats to e2m1, round to nearest even: v0 in the low nibble.
 __device__ __forceinline__ unsigned e2m1x8(float v0, float v1, float v2, float v3, float v4,
