@@ -148,56 +148,33 @@ __device__ __forceinline__ void color_of_record(const float* cam, const RawGauss
     }
 }
 
-// A warp's 32 colours through shared memory to `out` (its first Gaussian's):
-// of those in `mask`, or with ALL the first `left` floats.
-template <bool ALL>
-__device__ __forceinline__ void put_colors(float* out, float* s_col, const float col[3],
-                                           unsigned mask, int left)
-{
-    const int tid = threadIdx.x, lane = tid & 31, w0 = tid & ~31;
-#pragma unroll
-    for (int c = 0; c < 3; c++) s_col[3 * tid + c] = col[c];
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < 3; k++) {
-        const int e = 32 * k + lane;
-        if (ALL ? e < left : (mask >> (e / 3)) & 1u) out[e] = s_col[3 * w0 + e];
-    }
-    __syncwarp();
-}
-
-// Floats of a warp's colours that exist when its first Gaussian is i0.
-__device__ __forceinline__ int floats_left(long long n, long long i0)
-{
-    return (int)min(96LL, max(0LL, 3 * (n - i0)));
-}
-
 // One view.  Blocks stay and take every gridDim-th tile of kMxThreads
 // Gaussians; a tile's records load while the one before is computed, and its
-// radii, which say what of them to load, one tile earlier still.  1M Gaussians,
-// 60% visible: 13.7 us (a block per 256 Gaussians, all loads up front: 15.1; per
-// 128: 17.5).  Degree 4 would spill at the other degrees' 64 registers.
+// radii, which say what of them to load, one tile earlier still.  1M Gaussians:
+// 12.4 us, 60% of them visible 13.4 (a block per 256 Gaussians, all loads up
+// front: 15.1; per 128: 17.5).  Colours are stored where they are computed, three
+// floats a thread: whole lines by way of shared memory took longer (13.1; 8 views
+// of 6M 232), the L2 joins the parts.  Degree 4 would spill at the other degrees' 64 registers.
 constexpr int one_view_blocks(int deg) { return deg == 4 ? 6 : 8; }
 template <int DEG, int USE, bool MASKED>
 __global__ void __launch_bounds__(kMxThreads, one_view_blocks(DEG))
 mx4_colors_one_kernel(int n, const float* __restrict__ means, const void* __restrict__ records,
                       const Mx4Cam cam, const int* __restrict__ radii, float* __restrict__ colors)
 {
-    __shared__ float s_col[kMxThreads * 3];
     const long long step = (long long)gridDim.x * kMxThreads;
     long long i = (long long)blockIdx.x * kMxThreads + threadIdx.x;
     auto visible = [&](long long j) { return j < n && (!MASKED || radii[j] > 0); };
     bool on = visible(i), on_next = visible(i + step);
     RawGaussian<DEG> g, g_next;
     if (on) g.load(means, records, i);
-    for (; i - threadIdx.x < n; i += step) {
+    for (; i < n; i += step) {
         const bool on_after = visible(i + 2 * step);
         if (on_next) g_next.load(means, records, i + step);
         float col[3];
         color_of_record<DEG, USE>(cam.p, g, col);
-        const long long i0 = i - (threadIdx.x & 31);
-        const unsigned mask = MASKED ? __ballot_sync(0xffffffffu, on) : 0u;
-        put_colors<!MASKED>(colors + 3 * i0, s_col, col, mask, floats_left(n, i0));
+        if (on)
+#pragma unroll
+            for (int c = 0; c < 3; c++) colors[3 * i + c] = col[c];
         g = g_next;
         on = on_next;
         on_next = on_after;
@@ -206,24 +183,21 @@ mx4_colors_one_kernel(int n, const float* __restrict__ means, const void* __rest
 
 // Several views, one Gaussian a thread, its coefficients decoded once.  Bound
 // by arithmetic: at degree 3 about a hundred operations a colour.  8 views of
-// 6M Gaussians: 233 us (a pair of Gaussians a thread with the two-float
-// instructions: 226 to 261, their rate is the same).
+// 6M Gaussians: 210 us (a pair of Gaussians a thread in the two-float
+// instructions gained nothing, their rate is the same; nor did the basis'
+// constants multiplied into the coefficients, 221).
 template <int DEG, int USE, bool MASKED>
 __global__ void __launch_bounds__(kMxThreads)
 mx4_colors_kernel(int n, const float* __restrict__ means, const void* __restrict__ records,
                   int views, const Mx4Cams cams, const int* __restrict__ radii,
                   float* __restrict__ colors)
 {
-    __shared__ float s_col[kMxThreads * 3];
     const long long i = (long long)blockIdx.x * kMxThreads + threadIdx.x;
-    const long long i0 = i - (threadIdx.x & 31);
-    const int left = floats_left(n, i0);
+    if (i >= n) return;
     unsigned long long seen = 0;
     RawGaussian<DEG> g;
-    if (i < n) {  // most Gaussians have a view that sees them: no wait for the masks
-        g.load(means, records, i);
-        seen = MASKED ? views_of(radii, i, n, views) : ~0ull;
-    }
+    g.load(means, records, i);  // most Gaussians have a view that sees them: no wait for the masks
+    if (MASKED) seen = views_of(radii, i, n, views);
     float dc[3], s[3], q[3 * mx4_rest(DEG) + 1], col[3];
     mx4_dc(g.w, dc);
 #pragma unroll
@@ -233,10 +207,11 @@ mx4_colors_kernel(int n, const float* __restrict__ means, const void* __restrict
         mx4_codes<DEG>(g.w, q);
     }
     for (int v = 0; v < views; v++) {
-        const bool on = (seen >> v) & 1ull;
-        if (!MASKED || on) color_of<USE>(cams.p[v], g.p, q, s, dc, col);
-        const unsigned mask = MASKED ? __ballot_sync(0xffffffffu, on) : 0u;
-        put_colors<!MASKED>(colors + 3 * (v * (long long)n + i0), s_col, col, mask, left);
+        if (MASKED && !((seen >> v) & 1ull)) continue;
+        color_of<USE>(cams.p[v], g.p, q, s, dc, col);
+        float* out = colors + 3 * (v * (long long)n + i);
+#pragma unroll
+        for (int c = 0; c < 3; c++) out[c] = col[c];
     }
 }
 
