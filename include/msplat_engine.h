@@ -137,7 +137,10 @@ int msplat_train_step(
  *     with whole rows: key dropout_seed, counter (Gaussian, dropout_step))
  *     drops it takes no part in the step, as if the view culled it; the
  *     opacity of the others is multiplied by 1 / (1 - rate), in the gradient
- *     too.  Set dropout_step anew for each step.  The views of one step, and
+ *     too.  It may pass 1; alpha stays at most 0.999, and a pixel that it
+ *     brings there is replayed by the backward pass as it was blended, with a
+ *     gradient of the colour and none through alpha (a step without dropout
+ *     skips such a pixel, as the reference does).  Set dropout_step anew for each step.  The views of one step, and
  *     ranks, that are given the same seed and step drop the same Gaussians.
  *   mx4_colors  the forward pass takes its colours from 4-bit records of the
  *     features (see msplat_mx4_pack); gradients go straight through the

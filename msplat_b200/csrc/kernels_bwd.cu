@@ -69,6 +69,12 @@ struct PixelBwd {
 // skip decisions are the forward's (rasterize_backward_kernel :1023-1075).
 // v[3..5] are summed without the factor 0.5 and v[8] without the factor
 // -(1 - opacity); both are applied once after the warp reduction.
+// A pair at the cap of 0.999 is skipped whole in the plain step, as the
+// reference does it: a sigmoid reaches the cap next to never.  With DROPOUT the
+// opacity passes 1 and whole cores are at the cap, so such a pair is replayed as
+// the forward blended it -- T, the colour behind and the colour's gradient --
+// and only what goes through alpha, which the cap holds, has no gradient.
+template <bool DROPOUT>
 __device__ __forceinline__ bool backprop(PixelBwd& s, float fpx, float fpy, const float2 xy,
                                          const float4 co, const float4 rc, int idx, float v[9])
 {
@@ -79,10 +85,11 @@ __device__ __forceinline__ bool backprop(PixelBwd& s, float fpx, float fpy, cons
                              __fmul_rn(__fmul_rn(co.y, dx), dy));
     if (sigma < 0.f || sigma >= 5.55f) return false;
     const float alpha = fminf(0.999f, __fmul_rn(co.w, msp_expf_normal(-sigma)));
-    if (alpha < 1.f / 255.f || !(alpha < 0.999f)) return false;
+    const bool capped = !(alpha < 0.999f);
+    if (alpha < 1.f / 255.f || (!DROPOUT && capped)) return false;
     // 1 / (1 - alpha): the hardware reciprocal refined by one Newton step
     // (the product of these factors rebuilds T along the whole list, so a
-    // last-ulp bias would compound; d lies in (0.001, 1], no special cases)
+    // last-ulp bias would compound; d lies in [0.00099998, 1], no special cases)
     const float d = 1.f - alpha;
     const float r0 = __fdividef(1.f, d);
     const float ra = fmaf(r0, fmaf(-d, r0, 1.f), r0);
@@ -94,6 +101,7 @@ __device__ __forceinline__ bool backprop(PixelBwd& s, float fpx, float fpy, cons
     v[0] += fac * s.vo0;
     v[1] += fac * s.vo1;
     v[2] += fac * s.vo2;
+    if (DROPOUT && capped) return true;
     const float v_sigma = -alpha * v_alpha;
     v[3] += v_sigma * dxx;
     v[4] += v_sigma * (dx * dy);
@@ -269,7 +277,7 @@ raster_backward_kernel(const StepParams* __restrict__ P, const int* __restrict__
                 bool on = false;
 #pragma unroll
                 for (int h = 0; h < PPT; h++)
-                    on |= backprop(st[h], fpx, (float)(by + (lane >> 3) + 4 * h), xy, co, rc, idx, v);
+                    on |= backprop<DROPOUT>(st[h], fpx, (float)(by + (lane >> 3) + 4 * h), xy, co, rc, idx, v);
                 if (!__any_sync(0xffffffffu, on)) continue;
                 // Transposed butterfly: afterwards lane L holds the warp sum of
                 // value (L >> 2); the opacity term takes a plain butterfly.
