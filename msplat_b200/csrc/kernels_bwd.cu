@@ -113,7 +113,9 @@ __device__ __forceinline__ bool backprop(PixelBwd& s, float fpx, float fpy, cons
 }
 
 // DROPOUT: co.w is the sigmoid s times drop_scale, and the derivative with
-// respect to the logit needs 1 - s.
+// respect to the logit needs 1 - s.  Of an s that rounds to 1 the two roundings
+// on the way there and back can leave 1 - s below 0, a gradient of the wrong
+// sign that Adam would make a whole step of; it is at least 0.
 template <bool CHUNKED, int PPT, bool DROPOUT>
 __global__ void __launch_bounds__(256 / PPT, kBwdMinBlocks)
 raster_backward_kernel(const StepParams* __restrict__ P, const int* __restrict__ offset,
@@ -317,7 +319,7 @@ raster_backward_kernel(const StepParams* __restrict__ P, const int* __restrict__
                 } else if (lane == 1) {
                     if (vop != 0.f)
                         atomicAdd(grad_acc + (size_t)g * kGradStride + 8,
-                                  -(1.f - (DROPOUT ? co.w * P->drop_inv : co.w)) * vop);
+                                  -(DROPOUT ? fmaxf(1.f - co.w * P->drop_inv, 0.f) : 1.f - co.w) * vop);
                 }
             }
         }

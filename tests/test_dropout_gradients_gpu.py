@@ -91,6 +91,23 @@ def test_gradients_at_the_cap(n, w, h, spread, log_mu, chunked, rate):
     assert (np.abs(r["groups"][3][vis] - dc[vis]) <= bound[vis, :3] + 4 * rc.U * np.abs(dc[vis])).all()
 
 
+@pytest.mark.parametrize("rate", [0.05, 0.15, 0.2, 0.5])
+def test_a_saturated_sigmoid_has_no_gradient_of_the_wrong_sign(rate):
+    """Logits whose sigmoid rounds to 1: the derivative's factor 1 - s is at most
+    a few roundings of 1, and not negative."""
+    import torch
+    g, cs = scene(150, 320, 320, 0.7, 0.06, (17.5, 30.0), seed=150)
+    gt = torch.as_tensor(synthetic.target_image(320, 320, 1)).cuda()
+    r = run_step(g, cs, gt, rate)
+    want, bound, _, _, _ = rc.backward(
+        r["xy"].reshape(150, 2), r["conic"], r["opac"], r["rgb"], r["off"], r["ids"], 320, 320,
+        engine.DEFAULT_BG, r["v"], False)
+    sure = r["vis"] & (np.abs(want[:, 8]) > bound[:, 8])
+    assert sure.sum() >= 20
+    ratio = r["acc"][sure, 8] / want[sure, 8]
+    assert (ratio >= 0).all() and (ratio <= 4 * rc.U).all()
+
+
 def test_the_plain_step_skips_what_is_at_the_cap():
     """Without dropout a pair at the cap gives no gradient and does not count
     among what is behind (the reference's step): unlike the derivatives."""
