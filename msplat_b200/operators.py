@@ -18,6 +18,7 @@ from . import _lib
 REST_BASES = (0, 3, 8, 15, 24)      # SH coefficients beside dc, per channel, by degree
 RECORD_BYTES = (8, 16, 24, 32, 48)  # bytes of a Gaussian's record, by degree
 MAX_VIEWS = 64
+MAX_INT = 2**31 - 1                 # largest count that the C-ABI takes as an int
 
 # The current device's number and the handle of its current stream;
 # torch.cuda.current_stream() builds a Stream object around the latter, which
@@ -37,6 +38,12 @@ def _check(t, name: str, shape, dtype=torch.float32, device=None) -> None:
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+
+
+def _count(n: int, name: str) -> None:
+    """Refuses a count that the binding would cut down to 32 bits."""
+    if n > MAX_INT:
+        raise ValueError(f"{name} must be at most {MAX_INT}, not {n}")
 
 
 def _run(fn: str, device, *args) -> None:
@@ -79,6 +86,7 @@ def dropout(x, rate: float, seed: int, step: int, whole_rows: bool = False, out=
     if not 0.0 <= rate < 1.0:
         raise ValueError(f"the rate must be in [0, 1), not {rate}")
     rows, cols, xs = _rows(x, "x")
+    _count(cols, "the columns of x")
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
         ys = cols
@@ -112,6 +120,7 @@ def mx4_pack(features_dc, features_rest, out=None):
         raise ValueError("features_rest must be a tensor of shape (N, B, 3)")
     n, bases = features_rest.shape[:2]
     degree = _degree_of(bases)
+    _count(n, "the Gaussians")
     _check(features_rest, "features_rest", (n, bases, 3))
     dev = features_rest.device
     _check(features_dc, "features_dc", (n, 3), device=dev)
@@ -130,6 +139,7 @@ def _check_records(records, degree: int):
     if not isinstance(records, torch.Tensor) or records.dim() != 2:
         raise ValueError("records must be a tensor of shape (N, record bytes)")
     n = records.shape[0]
+    _count(n, "the Gaussians")
     _check(records, "records", (n, RECORD_BYTES[degree]), torch.uint8)
     return n, records.device
 
@@ -203,6 +213,7 @@ def mx4_colors_backward(v_colors, degree: int, means, cam_pos, degrees_to_use=No
     if not isinstance(means, torch.Tensor) or means.dim() != 2:
         raise ValueError("means must be a tensor of shape (N, 3)")
     n, dev = means.shape[0], means.device
+    _count(n, "the Gaussians")
     _check(means, "means", (n, 3))
     _check(v_colors, "v_colors", (views, n, 3), device=dev)
     rp = _radii(radii, views, n, dev)

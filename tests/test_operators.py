@@ -161,6 +161,33 @@ def test_python_refusals():
         operators.mx4_colors_backward(torch.zeros(1, 4, 3), 2, x, torch.zeros(1, 3))
 
 
+def test_counts_past_32_bits_are_refused(monkeypatch):
+    """The C-ABI takes columns and Gaussians as ints, which the binding would cut
+    down: 2^32 + 64 columns became 64.  Nothing may be called."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    calls = []
+    monkeypatch.setattr(operators, "_run", lambda fn, *a: calls.append(fn))
+    monkeypatch.setattr(torch.Tensor, "data_ptr", lambda t: 0)
+    with FakeTensorMode():
+        def cuda(*shape, dtype=torch.float32):
+            return torch.empty(*shape, dtype=dtype, device="cuda")
+        assert operators.dropout(cuda(2**32 + 64), 0.5, 1, 2).shape == (2**32 + 64,)     # rows are 64-bit
+        assert operators.dropout(cuda(1, 2**31 - 1), 0.5, 1, 2).shape == (1, 2**31 - 1)
+        assert calls == ["msplat_dropout"] * 2
+        calls.clear()
+        for n in (2**31, 2**32 + 64):
+            rec, means = cuda(n, 8, dtype=torch.uint8), cuda(n, 3)
+            for call in (lambda: operators.dropout(cuda(1, n), 0.5, 1, 2),
+                         lambda: operators.dropout(cuda(2, n + 3)[:, :n], 0.5, 1, 2, whole_rows=True),
+                         lambda: operators.mx4_pack(means, cuda(n, 0, 3)),
+                         lambda: operators.mx4_unpack(rec, 0),
+                         lambda: operators.mx4_colors(rec, 0, means, [[0, 0, 0]]),
+                         lambda: operators.mx4_colors_backward(cuda(1, n, 3), 0, means, [[0, 0, 0]])):
+                with pytest.raises(ValueError, match="at most"):
+                    call()
+    assert not calls
+
+
 # ---- options of the training step and the packed renderer
 
 def test_packed_scene_refusals():
