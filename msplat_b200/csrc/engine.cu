@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdarg>
 #include <cstddef>
 #include <cstdio>
@@ -101,12 +102,13 @@ struct Engine {
     std::vector<double> step_times;
     std::vector<double> stage_times[kStages];
     std::vector<int> pending_timing;  // ring slots with recorded events
-    long long launches = 0;
 
     cudaStream_t stream() const { return user_stream_set ? user_stream : own_stream; }
 };
 
 static Engine g;
+// For msplat_kernel_launches; counted outside the lock too (launched()).
+static std::atomic<long long> g_launches{0};
 // Device address of the counters that follow the parameters in d_slot.
 static int* d_counters()
 {
@@ -181,7 +183,7 @@ StepOptions swap_step_options(const StepOptions& o)
     g.opt = o;
     return before;
 }
-void engine_add_launches(int n) { g.launches += n; }
+void engine_add_launches(int n) { g_launches += n; }
 int launched(const char* who, int n)
 {
     const cudaError_t e = cudaGetLastError();
@@ -189,8 +191,7 @@ int launched(const char* who, int n)
         set_error("%s: %s", who, cudaGetErrorString(e));
         return MSPLAT_ERR_CUDA;
     }
-    std::lock_guard<std::mutex> lk(g_mu);
-    g.launches += n;
+    g_launches += n;  // no lock: an entry point may be waiting for the GPU under it
     return MSPLAT_OK;
 }
 
@@ -467,7 +468,7 @@ static int run_forward(const StepParams& p, const float* means, const float* sca
     g.last_num_tiles = p.num_tiles;
     g.last_prefix_sort = p.prefix_sort != 0;
     g.last_dense_bins = p.dense_bins != 0;
-    g.launches += 3 + sort_launches + (p.k_max > 1 ? 2 : p.prefix_sort ? 3 : 1);
+    g_launches += 3 + sort_launches + (p.k_max > 1 ? 2 : p.prefix_sort ? 3 : 1);
     MSP_CUDA(cudaGetLastError());
     return MSPLAT_OK;
 }
@@ -725,7 +726,7 @@ static int train_common(const char* who, int num_points, float* means3d, float* 
         bwd_launches = launch_project_backward_adam(g.d_params, num_points, p.degrees_to_use,
                                                     p.rest_stride, g.B, A, S, st);
     tm.mark(6, st);
-    g.launches += 1 + (p.k_max > 1 ? 2 : 1) + bwd_launches;
+    g_launches += 1 + (p.k_max > 1 ? 2 : 1) + bwd_launches;
     MSP_CUDA(cudaGetLastError());
     if ((rc = queue_readback(st, p))) return rc;
     if (radii_out) *radii_out = g.B.proj.radii;
@@ -945,7 +946,7 @@ int msplat_adam_apply(int num_points, int features_rest_bases, unsigned degree,
     a.begin = begin;
     a.end = end;
     launch_adam_apply(a, g.stream());
-    g.launches += 1;
+    g_launches += 1;
     MSP_CUDA(cudaGetLastError());
     return MSPLAT_OK;
 }
@@ -1122,10 +1123,7 @@ int msplat_count_raster_work(unsigned long long* out)
 
 long long msplat_kernel_launches(int reset)
 {
-    std::lock_guard<std::mutex> lk(g_mu);
-    long long n = g.launches;
-    if (reset) g.launches = 0;
-    return n;
+    return reset ? g_launches.exchange(0) : g_launches.load();
 }
 
 int msplat_last_binning(void)
