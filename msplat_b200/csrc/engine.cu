@@ -184,14 +184,14 @@ StepOptions swap_step_options(const StepOptions& o)
     return before;
 }
 void engine_add_launches(int n) { g_launches += n; }
-int launched(const char* who, int n)
+int launched(const char* who, cudaError_t e)
 {
-    const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
+        cudaGetLastError();  // reported here
         set_error("%s: %s", who, cudaGetErrorString(e));
         return MSPLAT_ERR_CUDA;
     }
-    g_launches += n;  // no lock: an entry point may be waiting for the GPU under it
+    g_launches += 1;  // no lock: an entry point may be waiting for the GPU under it
     return MSPLAT_OK;
 }
 

@@ -220,7 +220,19 @@ struct StepOptions {
 bool make_step_options(const char* who, double rate, unsigned long long seed,
                        unsigned long long step, bool mx4, StepOptions* out);
 StepOptions swap_step_options(const StepOptions& o);  // sets them; returns the earlier ones
-int launched(const char* who, int n);  // status after n launches of a call outside the lock; counts them
+int launched(const char* who, cudaError_t e);  // status of a launch outside the lock; counts it
+// Launches an operator's kernel.  The status is the launch's own: the runtime's
+// last error may be an earlier call's.
+template <typename... Params, typename... Args>
+int launch(const char* who, void (*kernel)(Params...), unsigned blocks, unsigned threads,
+           cudaStream_t s, Args&&... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    return launched(who, cudaLaunchKernelEx(&cfg, kernel, static_cast<Args&&>(args)...));
+}
 void stage_release();                // frees msplat_stage_input's buffers (engine lock held)
 
 // Host helpers shared by the entry points (engine.cu).

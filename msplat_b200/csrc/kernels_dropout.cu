@@ -262,9 +262,11 @@ extern "C" int msplat_dropout(long long rows, int cols, const float* x, long lon
     auto narrow = [&](long long per) {
         return (per / cols + 2) * std::max(x_stride, y_stride) < 1LL << 31;
     };
+    static const char* const who = "msplat_dropout";
+    int rc = MSPLAT_OK;
     if (whole_rows && cols > 1) {
         auto run = [&](auto kernel) {
-            kernel<<<blocks(kChunkElems), kDropThreads, 0, st>>>(a, total, magic);
+            rc = launch(who, kernel, blocks(kChunkElems), kDropThreads, st, a, total, magic);
         };
         auto pick = [&](auto R) {
             constexpr RowRule rule = R.value;
@@ -282,7 +284,7 @@ extern "C" int msplat_dropout(long long rows, int cols, const float* x, long lon
         const bool fits = cols > 1 && total < (1LL << 62) / cols;
         const unsigned long long magic64 = fits ? ~0ULL / (unsigned)cols + 1 : 0;
         auto run = [&](auto kernel) {
-            kernel<<<blocks(kElemsChunk), kDropThreads, 0, st>>>(a, total, magic, magic64);
+            rc = launch(who, kernel, blocks(kElemsChunk), kDropThreads, st, a, total, magic, magic64);
         };
         auto pick = [&](auto R) {
             constexpr RowRule rule = R.value;
@@ -297,5 +299,5 @@ extern "C" int msplat_dropout(long long rows, int cols, const float* x, long lon
         else if (cols == 1) pick(Rule<kOneColumn>());
         else magic ? pick(Rule<kByMagic>()) : pick(Rule<kWideRows>());
     }
-    return launched("msplat_dropout", 1);
+    return rc;
 }

@@ -90,11 +90,12 @@ int msplat_mx4_pack(int n, int degree, const float* features_dc, const float* fe
     if (!features_dc || (degree > 0 && !features_rest)) return mx4_null_pointer(who);
     if (!mx4_records_ok(who, records, degree)) return MSPLAT_ERR_ARG;
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+    int rc = MSPLAT_OK;
     with_degree(degree, [&](auto D) {
-        mx4_pack_kernel<D.value><<<mx4_blocks(n), kMxThreads, 0, st>>>(n, features_dc,
-                                                                        features_rest, records);
+        rc = launch(who, mx4_pack_kernel<D.value>, mx4_blocks(n), kMxThreads, st, n, features_dc,
+                    features_rest, records);
     });
-    return launched(who, 1);
+    return rc;
 }
 
 int msplat_mx4_unpack(int n, int degree, const void* records, float* features_dc,
@@ -106,11 +107,12 @@ int msplat_mx4_unpack(int n, int degree, const void* records, float* features_dc
     if (!features_dc || (degree > 0 && !features_rest)) return mx4_null_pointer(who);
     if (!mx4_records_ok(who, records, degree)) return MSPLAT_ERR_ARG;
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+    int rc = MSPLAT_OK;
     with_degree(degree, [&](auto D) {
-        mx4_unpack_kernel<D.value><<<mx4_blocks(n), kMxThreads, 0, st>>>(n, records, features_dc,
-                                                                          features_rest);
+        rc = launch(who, mx4_unpack_kernel<D.value>, mx4_blocks(n), kMxThreads, st, n, records,
+                    features_dc, features_rest);
     });
-    return launched(who, 1);
+    return rc;
 }
 
 }  // extern "C"

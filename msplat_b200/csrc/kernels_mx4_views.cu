@@ -320,22 +320,24 @@ int msplat_mx4_colors(int n, int degree, int degrees_to_use, const float* means3
     if (!means3d || !colors) return mx4_null_pointer(who);
     if (!mx4_records_ok(who, records, degree)) return MSPLAT_ERR_ARG;
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+    int rc = MSPLAT_OK;
     with_degrees(degree, degrees_to_use, [&](auto D, auto U) {
         constexpr int d = D.value, u = U.value;
         const unsigned tiles = mx4_blocks(n), stay = std::min(tiles, 148u * one_view_blocks(d));
         auto one = [&](auto kernel) {
             const Mx4Cam cam = {{cam_pos[0], cam_pos[1], cam_pos[2]}};
-            kernel<<<stay, kMxThreads, 0, st>>>(n, means3d, records, cam, radii, colors);
+            rc = launch(who, kernel, stay, kMxThreads, st, n, means3d, records, cam, radii, colors);
         };
         auto several = [&](auto kernel) {
-            kernel<<<tiles, kMxThreads, 0, st>>>(n, means3d, records, num_views, cams, radii, colors);
+            rc = launch(who, kernel, tiles, kMxThreads, st, n, means3d, records, num_views, cams,
+                        radii, colors);
         };
         if (num_views == 1)
             radii ? one(mx4_colors_one_kernel<d, u, true>) : one(mx4_colors_one_kernel<d, u, false>);
         else
             radii ? several(mx4_colors_kernel<d, u, true>) : several(mx4_colors_kernel<d, u, false>);
     });
-    return launched(who, 1);
+    return rc;
 }
 
 int msplat_mx4_colors_backward(int n, int degree, int degrees_to_use, const float* means3d,
@@ -353,15 +355,16 @@ int msplat_mx4_colors_backward(int n, int degree, int degrees_to_use, const floa
         (degree > 0 && !v_features_rest))
         return mx4_null_pointer(who);
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+    int rc = MSPLAT_OK;
     with_degrees(degree, degrees_to_use, [&](auto D, auto U) {
         auto run = [&](auto kernel) {
-            kernel<<<mx4_blocks(n), kMxThreads, 0, st>>>(n, means3d, num_views, cams, radii, v_colors,
-                                                         v_features_dc, v_features_rest);
+            rc = launch(who, kernel, mx4_blocks(n), kMxThreads, st, n, means3d, num_views, cams, radii,
+                        v_colors, v_features_dc, v_features_rest);
         };
         num_views == 1 ? run(mx4_colors_backward_kernel<D.value, U.value, 1>)
                        : run(mx4_colors_backward_kernel<D.value, U.value, 4>);
     });
-    return launched(who, 1);
+    return rc;
 }
 
 }  // extern "C"

@@ -66,3 +66,26 @@ def test_operators_do_not_wait_for_an_engine_call():
     assert before > 0
     operate()
     assert lib.msplat_kernel_launches(0) == 5
+
+
+def test_an_earlier_calls_failure_is_not_an_operators():
+    """An allocation that cannot be met fails by itself; the operators after it
+    give their results and no error."""
+    lib = _lib.load()
+    dc, rest = torch.randn(100, 3, device="cuda"), torch.randn(100, 15, 3, device="cuda")
+    g = torch.randn(2, 100, 3, device="cuda")
+    cams = [[0.0, 0.0, 9.0], [0.0, 9.0, 0.0]]
+
+    def calls():
+        rec = operators.mx4_pack(dc, rest)
+        yield from (rec, operators.dropout(rest, 0.5, 1, 2), operators.dropout(rest, 0.5, 1, 2, whole_rows=True),
+                    *operators.mx4_unpack(rec, 3), operators.mx4_colors(rec, 3, dc, cams),
+                    operators.mx4_colors(rec, 3, dc, cams[:1]),
+                    *operators.mx4_colors_backward(g, 3, dc, cams))
+    want = list(calls())
+    for f in (lambda: operators.mx4_pack(dc, rest), lambda: operators.dropout(rest, 0.5, 1, 2),
+              lambda: operators.mx4_colors(want[0], 3, dc, cams), lambda: list(calls())):
+        assert not lib.msplat_gpu_alloc(1 << 60, 0)
+        assert "failed" in lib.msplat_last_error().decode()
+        f()
+    assert all(torch.equal(a, b) for a, b in zip(want, calls()))
