@@ -176,13 +176,13 @@ bool make_step_options(const char* who, double rate, unsigned long long seed,
     return true;
 }
 
-StepOptions swap_step_options(const StepOptions& o)
-{
-    std::lock_guard<std::mutex> lk(g_mu);
-    const StepOptions before = g.opt;
-    g.opt = o;
-    return before;
-}
+// Options of the steps of this thread while a StepOptionsScope lives; else the
+// process's (g.opt).
+static thread_local const StepOptions* t_step_options = nullptr;
+StepOptionsScope::StepOptionsScope(const StepOptions& o) { t_step_options = &o; }
+StepOptionsScope::~StepOptionsScope() { t_step_options = nullptr; }
+static const StepOptions& step_options() { return t_step_options ? *t_step_options : g.opt; }
+
 void engine_add_launches(int n) { g_launches += n; }
 int launched(const char* who, cudaError_t e)
 {
@@ -445,13 +445,14 @@ static int run_forward(const StepParams& p, const float* means, const float* sca
                        bool train, StageMarks& tm, cudaStream_t st, const void* records = nullptr)
 {
     const Buffers& B = g.B;
+    const StepOptions& opt = step_options();
     const Colors colors = records ? Colors::kRecords
-                        : train && g.opt.mx4 ? Colors::kRounded : Colors::kFeatures;
+                        : train && opt.mx4 ? Colors::kRounded : Colors::kFeatures;
     tm.mark(0, st);
     launch_project_forward(g.d_params, p.num_points, means, scales, quats, dc,
                            records ? static_cast<const float*>(records) : rest, opac, B, train,
                            p.degrees_to_use, records ? mx4_words(p.degree) : p.rest_stride, st,
-                           colors, train && g.opt.dropout);
+                           colors, train && opt.dropout);
     tm.mark(1, st);
     launch_scan_tiles(g.d_params, p.num_tiles, p.dense_bins != 0, B, st);
     launch_scatter(g.d_params, p.num_points, B, st);
@@ -677,7 +678,8 @@ static int train_common(const char* who, int num_points, float* means3d, float* 
         set_error("%s: missing gt or statistics buffers", who);
         return MSPLAT_ERR_ARG;
     }
-    if (g.opt.mx4 && (degree > kMx4MaxDegree || features_rest_bases != mx4_rest((int)degree))) {
+    const StepOptions& opt = step_options();
+    if (opt.mx4 && (degree > kMx4MaxDegree || features_rest_bases != mx4_rest((int)degree))) {
         set_error("%s: 4-bit colours of SH degree %u need %d rest bases, not %d", who, degree,
                   degree > kMx4MaxDegree ? -1 : mx4_rest((int)degree), features_rest_bases);
         return MSPLAT_ERR_ARG;
@@ -699,11 +701,11 @@ static int train_common(const char* who, int num_points, float* means3d, float* 
     p.ssim_weight = ssim_weight;
     p.loss_inv_n = loss_inv_n;
     p.inv_max_dim = inv_max_dim;
-    p.drop_threshold = g.opt.threshold;
-    p.drop_seed = g.opt.seed;
-    p.drop_step = g.opt.step;
-    p.drop_scale = g.opt.scale;
-    p.drop_inv = (float)(1.0 - g.opt.threshold / 4294967296.0);
+    p.drop_threshold = opt.threshold;
+    p.drop_seed = opt.seed;
+    p.drop_step = opt.step;
+    p.drop_scale = opt.scale;
+    p.drop_inv = (float)(1.0 - opt.threshold / 4294967296.0);
     const cudaStream_t st = g.stream();
     if ((rc = ensure(num_points, img_width, img_height, p.num_tiles, p.k_max, true))) return rc;
     p.capacity = g.cap_isect;
@@ -715,7 +717,7 @@ static int train_common(const char* who, int num_points, float* means3d, float* 
     tm.mark(3, st);
     launch_ssim(g.d_params, p.img_w, p.img_h, gt, g.B, st);
     tm.mark(4, st);
-    launch_raster_backward(g.d_params, p.num_tiles, p.k_max, p.img_w, p.img_h, g.B, g.opt.dropout, st);
+    launch_raster_backward(g.d_params, p.num_tiles, p.k_max, p.img_w, p.img_h, g.B, opt.dropout, st);
     tm.mark(5, st);
     StatPtrs S{vis_counts, xys_grad_norm, max_2d_size};
     int bwd_launches = 1;
@@ -1031,7 +1033,8 @@ int msplat_set_step_options(const MsplatStepOptions* options)
                                       options->dropout_seed, options->dropout_step,
                                       options->mx4_colors != 0, &o))
         return MSPLAT_ERR_ARG;
-    swap_step_options(o);
+    std::lock_guard<std::mutex> lk(g_mu);
+    g.opt = o;
     return MSPLAT_OK;
 }
 

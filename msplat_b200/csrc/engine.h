@@ -219,7 +219,14 @@ struct StepOptions {
 };
 bool make_step_options(const char* who, double rate, unsigned long long seed,
                        unsigned long long step, bool mx4, StepOptions* out);
-StepOptions swap_step_options(const StepOptions& o);  // sets them; returns the earlier ones
+// While it lives, the steps that this thread calls take `o` and not the
+// process's options.
+struct StepOptionsScope {
+    explicit StepOptionsScope(const StepOptions& o);
+    ~StepOptionsScope();
+    StepOptionsScope(const StepOptionsScope&) = delete;
+    StepOptionsScope& operator=(const StepOptionsScope&) = delete;
+};
 int launched(const char* who, cudaError_t e);  // status of a launch outside the lock; counts it
 // Launches an operator's kernel.  The status is the launch's own: the runtime's
 // last error may be an earlier call's.

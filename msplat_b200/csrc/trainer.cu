@@ -487,13 +487,6 @@ struct TTrainer {
     }
 };
 
-// The trainer's own step options for the length of one step.
-struct StepOptionsScope {
-    StepOptions before;
-    explicit StepOptionsScope(const StepOptions& o) : before(swap_step_options(o)) {}
-    ~StepOptionsScope() { swap_step_options(before); }
-};
-
 MsplatPixelBuffer download_rgb(const float* dev, int w, int h)
 {
     MsplatPixelBuffer pb{nullptr, 0, 0};
