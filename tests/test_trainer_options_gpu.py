@@ -10,6 +10,7 @@ import pytest
 import msplat_b200 as msplat
 from msplat_b200 import _lib, engine, multigpu, synthetic
 from tests import dataset_case, harness
+from tests import operators_case as oc
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +66,26 @@ def test_two_trainers_in_two_threads(tmp_path):
             np.testing.assert_array_equal(p, q)
     a.close()
     b.close()
+
+
+def test_a_resumed_run_draws_as_an_uninterrupted_one(tmp_path):
+    """The iteration is the draws' step: after a checkpoint of iteration 6 both
+    the run and its resumption drop what step 7 drops, and go on so."""
+    t = trainer(tmp_path / "scene", dropout_rate=0.4, dropout_seed=5)
+    for _ in range(6):
+        t.step()
+    t.save_checkpoint(str(tmp_path / "a.msplat"))
+    u = trainer(tmp_path / "again", dropout_rate=0.4, dropout_seed=5)
+    u.load_checkpoint(str(tmp_path / "a.msplat"))
+    n = engine.GaussianModel.load_checkpoint(str(tmp_path / "a.msplat"))[0].n
+    for step in (7, 8):
+        kept, _ = oc.keep(np.arange(n), 0.4, step, 5)
+        for run in (t, u):
+            stats = run.step()
+            assert (stats.iteration, stats.splat_count) == (step, n)
+            r = radii(n)
+            # were another step's draws taken, each that the view sees would be
+            # one of ~kept with probability 0.4: none of 20, 4e-5
+            assert not r[~kept].any() and (r[kept] > 0).sum() >= 20
+    t.close()
+    u.close()
