@@ -328,6 +328,13 @@ struct Model {
 
     int render_mx4(const CamSetup& s, float** out)
     {
+        // a checkpoint may hold any number of bases; records hold whole degrees
+        const int bases = (s.degree + 1) * (s.degree + 1) - 1;
+        if (rest_bases != bases) {
+            set_error("4-bit colours of SH degree %d need %d rest bases, not %d", s.degree, bases,
+                      rest_bases);
+            return MSPLAT_ERR_ARG;
+        }
         const size_t bytes = (size_t)num_active * msplat_mx4_record_bytes(s.degree);
         if (bytes > records_bytes) {
             if (records) cudaFree(records);

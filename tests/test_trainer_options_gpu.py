@@ -89,3 +89,24 @@ def test_a_resumed_run_draws_as_an_uninterrupted_one(tmp_path):
             assert not r[~kept].any() and (r[kept] > 0).sum() >= 20
     t.close()
     u.close()
+
+
+def test_checkpoint_of_an_odd_number_of_bases(tmp_path):
+    """Ten rest bases are no whole SH degree, which records hold: a render, an
+    evaluation and a step with 4-bit colours say so."""
+    t = trainer(tmp_path / "scene")
+    t.step()
+    t.save_checkpoint(str(tmp_path / "a.msplat"))
+    model, step = engine.GaussianModel.load_checkpoint(str(tmp_path / "a.msplat"))
+    groups = [p.cpu().numpy() for p in model.params]
+    groups[4] = np.ascontiguousarray(groups[4][:, :10])
+    engine.GaussianModel(groups).save_checkpoint(str(tmp_path / "b.msplat"), step)
+    t.load_checkpoint(str(tmp_path / "b.msplat"))
+    t.set_options(mx4_colors=True)
+    with pytest.raises(RuntimeError, match="need 15 rest bases, not 10"):
+        t.render(0)
+    with pytest.raises(RuntimeError, match="rest bases"):
+        t.evaluate()
+    with pytest.raises(RuntimeError, match="rest bases"):
+        t.step()
+    t.close()
