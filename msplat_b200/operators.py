@@ -5,7 +5,9 @@ training step (engine.set_step_options) and the packed renderer
 Every call runs on torch's current stream of its tensors' device, allocates
 only its outputs (none where `out` is given) and does not wait.  Tensors are
 float32 unless stated; a wrong shape, type, layout or device raises
-ValueError before anything runs.  No counterpart in the reference.
+ValueError before anything runs.  Autograd does not record the calls: a tensor
+that requires a gradient is refused unless gradients are off (torch.no_grad());
+the backward passes are calls of their own.  No counterpart in the reference.
 """
 from __future__ import annotations
 
@@ -29,7 +31,7 @@ _stream_of = torch._C._cuda_getCurrentRawStream
 
 def _check(t, name: str, shape, dtype=torch.float32, device=None) -> None:
     if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and t.shape == shape
-            and t.is_contiguous() and (device is None or t.device == device)):
+            and t.is_contiguous() and (device is None or t.device == device) and not t.requires_grad):
         return
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor of {dtype}")
@@ -37,7 +39,15 @@ def _check(t, name: str, shape, dtype=torch.float32, device=None) -> None:
         raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+    _unrecorded(t, name)
+
+
+def _unrecorded(t, name: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which this call does not record: "
+                         "call it under torch.no_grad(), and its backward pass on the gradient")
 
 
 def _count(n: int, name: str) -> None:
@@ -85,6 +95,7 @@ def dropout(x, rate: float, seed: int, step: int, whole_rows: bool = False, out=
         raise ValueError("x must be a CUDA tensor of torch.float32")
     if not 0.0 <= rate < 1.0:
         raise ValueError(f"the rate must be in [0, 1), not {rate}")
+    _unrecorded(x, "x")
     rows, cols, xs = _rows(x, "x")
     _count(cols, "the columns of x")
     if out is None:
@@ -95,6 +106,7 @@ def dropout(x, rate: float, seed: int, step: int, whole_rows: bool = False, out=
             raise ValueError("out must be a float32 tensor on x's device")
         if out.shape != x.shape:
             raise ValueError(f"out must have shape {tuple(x.shape)}, not {tuple(out.shape)}")
+        _unrecorded(out, "out")
         ys = _rows(out, "out")[2]
     if rows and cols:
         _run("msplat_dropout", x.device, rows, cols, x.data_ptr(), xs, out.data_ptr(), ys, rate,

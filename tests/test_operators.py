@@ -188,6 +188,58 @@ def test_counts_past_32_bits_are_refused(monkeypatch):
     assert not calls
 
 
+@pytest.fixture
+def fake_cuda(monkeypatch):
+    """CUDA tensors without memory, and the calls that would have been made."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    calls = []
+    monkeypatch.setattr(operators, "_run", lambda fn, *a: calls.append(fn))
+    monkeypatch.setattr(torch.Tensor, "data_ptr", lambda t: 0)
+    with FakeTensorMode():
+        yield calls
+
+
+def operator_calls(grad=(), out=False):
+    """Each operator's call with its tensors by name; those in `grad` require a
+    gradient."""
+    def t(name, *shape, dtype=torch.float32):
+        return torch.empty(*shape, dtype=dtype, device="cuda", requires_grad=name in grad)
+    rec, means, cams = t("records", 9, 32, dtype=torch.uint8), t("means", 9, 3), [[0, 0, 9]]
+    dc, rest = t("dc", 9, 3), t("rest", 9, 15, 3)
+    outs = dict(y=t("y", 9, 3), rec=torch.empty(9, 32, dtype=torch.uint8, device="cuda"), pair=(t("out0", 9, 3), t("out1", 9, 15, 3)),
+                colors=t("out", 1, 9, 3))
+
+    def kw(name):
+        return dict(out=outs[name]) if out else {}
+    return outs, {
+        "dropout": (("x",), lambda: operators.dropout(t("x", 9, 3), 0.5, 1, 2, **kw("y"))),
+        "mx4_pack": (("dc", "rest"), lambda: operators.mx4_pack(dc, rest, **kw("rec"))),
+        "mx4_unpack": ((), lambda: operators.mx4_unpack(rec, 3, **kw("pair"))),
+        "mx4_colors": (("means",), lambda: operators.mx4_colors(rec, 3, means, cams, **kw("colors"))),
+        "mx4_colors_backward": (("v", "means"), lambda: operators.mx4_colors_backward(
+            t("v", 1, 9, 3), 3, means, cams, **kw("pair")))}
+
+
+def test_inputs_that_require_a_gradient_are_refused(fake_cuda):
+    """Autograd would not hear of the call: its result would be a constant to
+    the graph.  Without gradients the call is made."""
+    for name, (inputs, _) in operator_calls()[1].items():
+        for i in inputs:
+            call = operator_calls(grad=(i,))[1][name][1]
+            with pytest.raises(ValueError, match="requires a gradient"):
+                call()
+            assert not fake_cuda
+            with torch.no_grad():
+                assert not any(o.requires_grad for o in (call(),) if isinstance(o, torch.Tensor))
+            assert fake_cuda == ["msplat_" + name]
+            fake_cuda.clear()
+    for name, o in (("dropout", "y"), ("mx4_unpack", "out0"), ("mx4_unpack", "out1"), ("mx4_colors", "out"),
+                    ("mx4_colors_backward", "out1")):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            operator_calls(grad=(o,), out=True)[1][name][1]()
+    assert not fake_cuda
+
+
 # ---- options of the training step and the packed renderer
 
 def test_packed_scene_refusals():
