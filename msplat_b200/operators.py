@@ -7,7 +7,8 @@ only its outputs (none where `out` is given) and does not wait.  Tensors are
 float32 unless stated; a wrong shape, type, layout or device raises
 ValueError before anything runs.  Autograd does not record the calls: a tensor
 that requires a gradient is refused unless gradients are off (torch.no_grad());
-the backward passes are calls of their own.  No counterpart in the reference.
+the backward passes are calls of their own.  What is written into `out` counts
+as modified in place.  No counterpart in the reference.
 """
 from __future__ import annotations
 
@@ -48,6 +49,10 @@ def _unrecorded(t, name: str) -> None:
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which this call does not record: "
                          "call it under torch.no_grad(), and its backward pass on the gradient")
+
+
+# For outputs that the caller handed in.
+_written = torch.autograd.graph.increment_version
 
 
 def _count(n: int, name: str) -> None:
@@ -108,6 +113,7 @@ def dropout(x, rate: float, seed: int, step: int, whole_rows: bool = False, out=
             raise ValueError(f"out must have shape {tuple(x.shape)}, not {tuple(out.shape)}")
         _unrecorded(out, "out")
         ys = _rows(out, "out")[2]
+        _written(out)
     if rows and cols:
         _run("msplat_dropout", x.device, rows, cols, x.data_ptr(), xs, out.data_ptr(), ys, rate,
              int(seed) & (2**64 - 1), int(step) & (2**64 - 1), int(bool(whole_rows)))
@@ -141,6 +147,7 @@ def mx4_pack(features_dc, features_rest, out=None):
         out = features_dc.new_empty(shape, dtype=torch.uint8)
     else:
         _check(out, "out", shape, torch.uint8, dev)
+        _written(out)
     _run("msplat_mx4_pack", dev, n, degree, features_dc.data_ptr(), features_rest.data_ptr(),
          out.data_ptr())
     return out
@@ -166,6 +173,7 @@ def mx4_unpack(records, degree: int, out=None):
     else:
         for t, s, name in zip(out, shapes, ("out[0]", "out[1]"), strict=True):
             _check(t, name, s, device=dev)
+        _written(out)
     _run("msplat_mx4_unpack", dev, n, degree, records.data_ptr(), out[0].data_ptr(),
          out[1].data_ptr())
     return out
@@ -209,6 +217,7 @@ def mx4_colors(records, degree: int, means, cam_pos, degrees_to_use=None, radii=
         out = (means.new_empty if radii is None else means.new_zeros)((views, n, 3))
     else:
         _check(out, "out", (views, n, 3), device=dev)
+        _written(out)
     _run("msplat_mx4_colors", dev, n, degree, use, means.data_ptr(), records.data_ptr(), views,
          cams, rp, out.data_ptr())
     return out
@@ -235,6 +244,7 @@ def mx4_colors_backward(v_colors, degree: int, means, cam_pos, degrees_to_use=No
     else:
         for t, s, name in zip(out, shapes, ("out[0]", "out[1]"), strict=True):
             _check(t, name, s, device=dev)
+        _written(out)
     _run("msplat_mx4_colors_backward", dev, n, degree, use, means.data_ptr(), views,
          cams, rp, v_colors.data_ptr(), out[0].data_ptr(), out[1].data_ptr())
     return out

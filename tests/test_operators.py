@@ -240,6 +240,22 @@ def test_inputs_that_require_a_gradient_are_refused(fake_cuda):
     assert not fake_cuda
 
 
+def test_outputs_that_were_handed_in_count_as_modified(fake_cuda):
+    """A graph that saved such a tensor must learn that it changed."""
+    for name, written in (("dropout", ("y",)), ("mx4_pack", ("rec",)), ("mx4_unpack", ("pair",)),
+                          ("mx4_colors", ("colors",)), ("mx4_colors_backward", ("pair",))):
+        outs, calls = operator_calls(out=True)
+
+        def versions():
+            return {k: [u._version for u in (v if isinstance(v, tuple) else (v,))] for k, v in outs.items()}
+        before = versions()
+        calls[name][1]()
+        after = versions()
+        for k in outs:
+            assert (after[k] == [v + 1 for v in before[k]]) == (k in written), (name, k)
+            assert k in written or after[k] == before[k]
+
+
 # ---- options of the training step and the packed renderer
 
 def test_packed_scene_refusals():
