@@ -339,10 +339,11 @@ class PackedGaussians:
 
     def __init__(self, means, scales, quats, opacities, records, sh_degree: int):
         from . import operators
-        n, dev = operators._check_records(records, sh_degree)
-        for t, name, width in ((means, "means", 3), (scales, "scales", 3), (quats, "quats", 4),
-                               (opacities, "opacities", 1)):
-            operators._check(t, name, (n, width), device=dev)
+        with _torch().no_grad():   # a scene to render: no gradient is expected of it
+            n, dev = operators._check_records(records, sh_degree)
+            for t, name, width in ((means, "means", 3), (scales, "scales", 3), (quats, "quats", 4),
+                                   (opacities, "opacities", 1)):
+                operators._check(t, name, (n, width), device=dev)
         self.means, self.scales, self.quats, self.opacities = means, scales, quats, opacities
         self.records, self.sh_degree = records, int(sh_degree)
 

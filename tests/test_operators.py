@@ -240,6 +240,14 @@ def test_inputs_that_require_a_gradient_are_refused(fake_cuda):
     assert not fake_cuda
 
 
+def test_a_packed_scene_takes_parameters(fake_cuda):
+    """A scene to render may hold tensors that require a gradient."""
+    from msplat_b200 import engine
+    t = [torch.empty(9, w, device="cuda", requires_grad=True) for w in (3, 3, 4, 1)]
+    packed = engine.PackedGaussians(*t, torch.empty(9, 32, dtype=torch.uint8, device="cuda"), 3)
+    assert packed.n == 9 and packed.means is t[0]
+
+
 def test_outputs_that_were_handed_in_count_as_modified(fake_cuda):
     """A graph that saved such a tensor must learn that it changed."""
     for name, written in (("dropout", ("y",)), ("mx4_pack", ("rec",)), ("mx4_unpack", ("pair",)),
