@@ -12,7 +12,6 @@ as modified in place.  No counterpart in the reference.
 """
 from __future__ import annotations
 
-
 import numpy as np
 import torch
 
@@ -25,9 +24,10 @@ MAX_INT = 2**31 - 1                 # largest count that the C-ABI takes as an i
 
 # The current device's number and the handle of its current stream;
 # torch.cuda.current_stream() builds a Stream object around the latter, which
-# took 3.2 us of a 14 us call.
-_device_now = torch._C._cuda_getDevice
-_stream_of = torch._C._cuda_getCurrentRawStream
+# took 3.2 us of a 14 us call.  (A torch without CUDA has neither, and no
+# tensor that passes the checks.)
+_device_now = getattr(torch._C, "_cuda_getDevice", None)
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _check(t, name: str, shape, dtype=torch.float32, device=None) -> None:

@@ -5,6 +5,8 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -186,6 +188,18 @@ def test_counts_past_32_bits_are_refused(monkeypatch):
                 with pytest.raises(ValueError, match="at most"):
                     call()
     assert not calls
+
+
+def test_a_torch_without_cuda_can_import_the_module():
+    code = ("import torch\n"
+            "for name in ('_cuda_getDevice', '_cuda_getCurrentRawStream'):\n"
+            "    if hasattr(torch._C, name): delattr(torch._C, name)\n"
+            "from msplat_b200 import operators\n"
+            "try: operators.dropout(torch.zeros(3), 0.5, 1, 2)\n"
+            "except ValueError as e: assert 'CUDA tensor' in str(e)\n"
+            "else: raise AssertionError\n")
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300,
+                   cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 
 @pytest.fixture
