@@ -18,7 +18,7 @@ constexpr int kDropThreads = 256;
 struct DropArgs {
     const float* x;
     float* y;
-    long long rows, x_stride, y_stride;
+    long long x_stride, y_stride;
     int cols;
     unsigned threshold;
     float scale;
@@ -248,7 +248,7 @@ extern "C" int msplat_dropout(long long rows, int cols, const float* x, long lon
                                                  : "in place needs the same row stride twice");
         return MSPLAT_ERR_ARG;
     }
-    const DropArgs a{x, y, rows, x_stride, y_stride, cols, dr.threshold, dr.scale, step, philox_keys(seed)};
+    const DropArgs a{x, y, x_stride, y_stride, cols, dr.threshold, dr.scale, step, philox_keys(seed)};
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     const long long total = rows * cols;
     const bool xgaps = x_stride != cols, ygaps = y_stride != cols, flat = !xgaps && !ygaps;

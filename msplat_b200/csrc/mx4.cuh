@@ -1,6 +1,7 @@
 // mx4.cuh -- 4-bit colour records: a Gaussian's SH coefficients in one small
-// aligned record, microscaled as the OCP MX formats are (e2m1 elements under
-// a power-of-two e8m0 scale), with one block per colour channel.
+// aligned record, with the element and scale types of the OCP MX formats (e2m1
+// under a power-of-two e8m0 scale), but a block per colour channel (3 to 24
+// elements, not 32) and another choice of the scale (below).
 //
 // Record of SH degree D with B = (D+1)^2 - 1 rest coefficients per channel
 // (8, 16, 24, 32, 48 bytes for D = 0..4; degree 3 is one 32-byte sector):
@@ -229,21 +230,7 @@ __device__ __forceinline__ void mx4_store(void* records, long long i,
     }
 }
 
-// Unit direction from a camera to a mean.
-__device__ __forceinline__ void view_dir(const float* cam, const float p[3], float d[3])
-{
-    const float d0 = p[0] - cam[0], d1 = p[1] - cam[1], d2 = p[2] - cam[2];
-    const float dn = rsqrt_ieee((d0 * d0 + d1 * d1) + d2 * d2);
-    d[0] = d0 * dn;
-    d[1] = d1 * dn;
-    d[2] = d2 * dn;
-}
-
-// Colour of one channel: dc and code sums per degree.  The products and
-// sums are sh_to_color's (kernels_fwd.cu) in its order on the codes; the
-// power-of-two scale commutes with every rounding (short of overflow and
-// underflow), so a colour is bit for bit what the projection computes from
-// the unpacked coefficients.
+// A unit direction and the products of its components.
 struct ShDir {
     float x, y, z, xx, xy, xz, yy, yz, zz;
 };
@@ -254,6 +241,11 @@ __device__ __forceinline__ ShDir sh_dir(const float d[3])
             d[2] * d[2]};
 }
 
+// Colour of one channel: dc and code sums per degree.  The products and
+// sums are sh_to_color's (kernels_fwd.cu) in its order on the codes; the
+// power-of-two scale commutes with every rounding (short of overflow and
+// underflow), so a colour is bit for bit what the projection computes from
+// the unpacked coefficients.
 // `r(k)`: coefficient k of the channel, unscaled.
 template <int DEG, typename R>
 __device__ __forceinline__ float mx4_color(int use, const ShDir& D, float dc, float scale, R r)
