@@ -323,8 +323,9 @@ int msplat_mx4_colors(int n, int degree, int degrees_to_use, const float* means3
     int rc = MSPLAT_OK;
     with_degrees(degree, degrees_to_use, [&](auto D, auto U) {
         constexpr int d = D.value, u = U.value;
-        const unsigned tiles = mx4_blocks(n), stay = std::min(tiles, 148u * one_view_blocks(d));
+        const unsigned tiles = mx4_blocks(n);
         auto one = [&](auto kernel) {
+            const unsigned stay = std::min(tiles, (unsigned)(device_sms() * one_view_blocks(d)));
             const Mx4Cam cam = {{cam_pos[0], cam_pos[1], cam_pos[2]}};
             rc = launch(who, kernel, stay, kMxThreads, st, n, means3d, records, cam, radii, colors);
         };
