@@ -165,7 +165,7 @@ mx4_colors_one_kernel(int n, const float* __restrict__ means, const void* __rest
     long long i = (long long)blockIdx.x * kMxThreads + threadIdx.x;
     auto visible = [&](long long j) { return j < n && (!MASKED || radii[j] > 0); };
     bool on = visible(i), on_next = visible(i + step);
-    RawGaussian<DEG> g, g_next;
+    RawGaussian<DEG> g{}, g_next{};  // set, as lanes that are off compute too
     if (on) g.load(means, records, i);
     for (; i < n; i += step) {
         const bool on_after = visible(i + 2 * step);
