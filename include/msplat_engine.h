@@ -289,7 +289,8 @@ int msplat_render(
  * Forward-only render of a scene whose colours are 4-bit records
  * (msplat_mx4_pack with SH degree `degree`, 0 to 4): msplat_render with
  * `records` for features_dc and features_rest, and the image that it would
- * give for the unpacked features, bit for bit.
+ * give for the unpacked features, bit for bit (while no colour's sum
+ * overflows: coefficients far below 1e38).
  */
 int msplat_render_mx4(
     int num_points, const float *means3d, const float *scales, float glob_scale,
@@ -600,8 +601,8 @@ int msplat_dropout(long long rows, int cols, const float *x, long long x_stride,
  * the order of features_rest [B,3]; the last bytes are zero.  A channel's
  * scale puts its largest magnitude in [3.5, 7), so that every coefficient is
  * within half a step of the e2m1 grid; coefficients round to nearest, ties to
- * even (from 7 * 2^125 on they saturate at 6 * 2^125).  A NaN or an infinity makes its channel of that Gaussian NaN
- * (b = 255); dc beyond 65504 becomes infinite.  Record arrays are aligned to
+ * even (from 7 * 2^125 on they saturate at 6 * 2^125).  A NaN or an infinity
+ * makes its channel of that Gaussian NaN (b = 255); dc beyond 65504 becomes infinite.  Record arrays are aligned to
  * 16 bytes (8 at degrees 0 and 2). */
 int msplat_mx4_record_bytes(int degree);
 

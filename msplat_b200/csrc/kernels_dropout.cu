@@ -52,9 +52,10 @@ __device__ __forceinline__ int local_row(unsigned t, int cols, unsigned magic)
 // lane's own four.  Offset: the type that holds a row offset in a chunk (32
 // bits for all but the widest strides); YGAPS: y's rows are apart.  40M
 // elements without gaps: 54 us (5.9 TB/s), at any alignment -- a vector an access
-// is no faster.  With gaps it is bound by instructions, the draws' and the
-// indexes': 333,337 rows of 23 in rows of 27, 15.2 us a pass (4.0 TB/s).  48
-// registers: 18.1 us where 78 took 21.4.
+// is no faster.  With gaps it is bound by the pipe of the draws' wide
+// multiplications, which is busy two thirds of the time that the
+// multiprocessors are: 333,337 rows of 23 in rows of 27, 15.2 us a pass
+// (4.0 TB/s).  48 registers: 18.1 us where 78 took 21.4.
 // `magic64` = ceil(2^64 / cols) divides the chunk's first index exactly while
 // index * cols < 2^64; 0: plain division.
 constexpr int kElemsChunk = 256 * (kDropThreads / 32);

@@ -182,8 +182,9 @@ mx4_colors_one_kernel(int n, const float* __restrict__ means, const void* __rest
 }
 
 // Several views, one Gaussian a thread, its coefficients decoded once.  Bound
-// by arithmetic: at degree 3 about a hundred operations a colour.  8 views of
-// 6M Gaussians: 210 us (a pair of Gaussians a thread in the two-float
+// by instructions (82% of the issue slots at degree 3): 135 a colour, of which
+// direction, basis and product are about a hundred.  8 views of 6M Gaussians:
+// 210 us (a pair of Gaussians a thread in the two-float
 // instructions gained nothing, their rate is the same; nor did the basis'
 // constants multiplied into the coefficients, 221).
 template <int DEG, int USE, bool MASKED>

@@ -8,7 +8,8 @@ float32 unless stated; a wrong shape, type, layout or device raises
 ValueError before anything runs.  Autograd does not record the calls: a tensor
 that requires a gradient is refused unless gradients are off (torch.no_grad());
 the backward passes are calls of their own.  What is written into `out` counts
-as modified in place.  No counterpart in the reference.
+as modified in place; it must not overlap an input (but dropout works in
+place).  No counterpart in the reference.
 """
 from __future__ import annotations
 
