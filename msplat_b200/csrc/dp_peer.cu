@@ -475,6 +475,7 @@ std::map<std::string, void*> g_opened;  // IPC handle bytes -> mapped pointer
     do {                                                                                  \
         cudaError_t e_ = (expr);                                                          \
         if (e_ != cudaSuccess) {                                                          \
+            cudaGetLastError(); /* reported here, not by the next call */                 \
             set_error("%s failed: %s", #expr, cudaGetErrorString(e_));                    \
             return MSPLAT_ERR_CUDA;                                                       \
         }                                                                                 \

@@ -40,6 +40,7 @@ void set_error(const char* fmt, ...)
     do {                                                                                  \
         cudaError_t e_ = (expr);                                                          \
         if (e_ != cudaSuccess) {                                                          \
+            cudaGetLastError(); /* reported here, not by the next call */                 \
             set_error("%s failed: %s (%s:%d)", #expr, cudaGetErrorString(e_), __FILE__,   \
                       __LINE__);                                                          \
             return MSPLAT_ERR_CUDA;                                                       \
@@ -524,6 +525,7 @@ void* msplat_gpu_alloc(size_t bytes, int zero)
     if (init_engine()) return nullptr;
     void* p = nullptr;
     if (cudaMalloc(&p, bytes ? bytes : 4) != cudaSuccess) {
+        cudaGetLastError();
         set_error("cudaMalloc(%zu) failed", bytes);
         return nullptr;
     }
@@ -547,6 +549,7 @@ void* msplat_shared_alloc(size_t bytes, int zero)
     const size_t n = bytes ? bytes : 4;
     cudaError_t e = cudaMallocManaged(&p, n, cudaMemAttachGlobal);
     if (e != cudaSuccess) {
+        cudaGetLastError();
         set_error("cudaMallocManaged(%zu) failed: %s", n, cudaGetErrorString(e));
         return nullptr;
     }

@@ -152,6 +152,7 @@ __global__ void knn_query_kernel(const float4* __restrict__ sorted, long long n,
     do {                                                                                \
         cudaError_t e_ = (expr);                                                        \
         if (e_ != cudaSuccess) {                                                        \
+            cudaGetLastError(); /* reported here, not by the next call */               \
             set_error("msplat_knn_mean_distance: %s: %s", #expr, cudaGetErrorString(e_)); \
             rc = MSPLAT_ERR_CUDA;                                                       \
             goto done;                                                                  \

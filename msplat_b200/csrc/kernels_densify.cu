@@ -300,6 +300,7 @@ int grow(void** p, long long& cap, long long want, size_t elem)
     *p = nullptr;
     cap = 0;
     if (cudaMalloc(p, (size_t)std::max(want, 1LL) * elem) != cudaSuccess) {
+        cudaGetLastError();
         set_error("msplat_densify: cudaMalloc of %lld scratch elements failed", want);
         return MSPLAT_ERR_CUDA;
     }
@@ -311,6 +312,7 @@ int grow(void** p, long long& cap, long long want, size_t elem)
     do {                                                                                  \
         cudaError_t e_ = (expr);                                                          \
         if (e_ != cudaSuccess) {                                                          \
+            cudaGetLastError(); /* reported here, not by the next call */                 \
             set_error("msplat_densify: %s failed: %s", #expr, cudaGetErrorString(e_));    \
             return MSPLAT_ERR_CUDA;                                                       \
         }                                                                                 \

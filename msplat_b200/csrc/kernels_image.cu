@@ -27,6 +27,7 @@ namespace {
     do {                                                                                 \
         cudaError_t e_ = (expr);                                                         \
         if (e_ != cudaSuccess) {                                                         \
+            cudaGetLastError(); /* reported here, not by the next call */                \
             set_error("%s failed: %s", #expr, cudaGetErrorString(e_));                   \
             return MSPLAT_ERR_CUDA;                                                      \
         }                                                                                \

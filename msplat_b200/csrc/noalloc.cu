@@ -121,6 +121,7 @@ int scratch_base(void** base)
     do {                                                                                  \
         cudaError_t e_ = (expr);                                                          \
         if (e_ != cudaSuccess) {                                                          \
+            cudaGetLastError(); /* reported here, not by the next call */                 \
             set_error("msplat_render_noalloc: %s failed: %s", #expr, cudaGetErrorString(e_)); \
             return MSPLAT_ERR_CUDA;                                                       \
         }                                                                                 \

@@ -41,6 +41,7 @@ Stage s_stage;
     do {                                                                               \
         cudaError_t e_ = (expr);                                                       \
         if (e_ != cudaSuccess) {                                                       \
+            cudaGetLastError(); /* reported here, not by the next call */              \
             set_error("msplat_stage_input: %s: %s", #expr, cudaGetErrorString(e_));   \
             return MSPLAT_ERR_CUDA;                                                    \
         }                                                                              \

@@ -89,3 +89,17 @@ def test_an_earlier_calls_failure_is_not_an_operators():
         assert "failed" in lib.msplat_last_error().decode()
         f()
     assert all(torch.equal(a, b) for a, b in zip(want, calls()))
+
+
+def test_a_failed_allocation_is_reported_once():
+    """It does not come up again as a render's or a step's error."""
+    engine.bind_stream()
+    lib = _lib.load()
+    gt = torch.as_tensor(synthetic.target_image(64, 48, 1)).cuda()
+    model = engine.GaussianModel(synthetic.gaussians(500, 1).groups())
+    cs = harness.setup_cam(synthetic.front_camera(64, 48, 3.0))
+    for alloc in (lib.msplat_gpu_alloc, lib.msplat_shared_alloc):
+        for call in (lambda: engine.render(model, cs), lambda: engine.train_step(model, cs, gt)):
+            assert not alloc(1 << 60, 0)
+            call()
+    torch.cuda.synchronize()
