@@ -193,7 +193,7 @@ def _views(cam_pos):
 def _use(degrees_to_use, degree: int) -> int:
     if degrees_to_use is None:
         return degree
-    if not 0 <= degrees_to_use <= degree:
+    if degrees_to_use not in range(degree + 1):
         raise ValueError(f"degrees_to_use must be 0 to {degree}, not {degrees_to_use}")
     return int(degrees_to_use)
 

@@ -163,6 +163,16 @@ def test_python_refusals():
         operators.mx4_colors_backward(torch.zeros(1, 4, 3), 2, x, torch.zeros(1, 3))
 
 
+@pytest.mark.parametrize("use", [-1, 4, 1.5, 2.999, float("nan")])
+def test_degrees_to_use_that_are_none(use):
+    with pytest.raises(ValueError, match="degrees_to_use"):
+        operators._use(use, 3)
+
+
+def test_degrees_to_use():
+    assert [operators._use(u, 3) for u in (None, 0, 3, np.int64(2), 1.0)] == [3, 0, 3, 2, 1]
+
+
 def test_counts_past_32_bits_are_refused(monkeypatch):
     """The C-ABI takes columns and Gaussians as ints, which the binding would cut
     down: 2^32 + 64 columns became 64.  Nothing may be called."""
