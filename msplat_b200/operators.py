@@ -78,6 +78,8 @@ def _rows(t, name: str):
     """A tensor as (rows, cols, row stride): two dimensions with unit column
     stride, or contiguous of any number of dimensions (rows of the last
     one; one column where there is a single dimension)."""
+    if t.is_neg():   # the sign is not in memory yet
+        raise ValueError(f"{name} is a negated view: pass {name}.resolve_neg()")
     if t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1):
         rows, cols = t.shape
         stride = t.stride(0) if rows > 1 else max(cols, 1)

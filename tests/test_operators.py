@@ -163,6 +163,14 @@ def test_python_refusals():
         operators.mx4_colors_backward(torch.zeros(1, 4, 3), 2, x, torch.zeros(1, 3))
 
 
+def test_a_negated_view_is_refused():
+    """The imaginary part of a conjugate: its memory holds the other sign."""
+    x = torch.complex(torch.ones(4, 1), torch.ones(4, 1)).conj().imag
+    with pytest.raises(ValueError, match="negated"):
+        operators._rows(x, "x")
+    assert operators._rows(x.resolve_neg(), "x") == (4, 1, 1)
+
+
 @pytest.mark.parametrize("use", [-1, 4, 1.5, 2.999, float("nan")])
 def test_degrees_to_use_that_are_none(use):
     with pytest.raises(ValueError, match="degrees_to_use"):
