@@ -246,7 +246,6 @@ void stage_release();                // frees msplat_stage_input's buffers (engi
 void set_error(const char* fmt, ...);                  // text for msplat_last_error()
 int fill_params(StepParams& p, const CamArgs& a);      // validates, fills the block
 int chunk_k_max(long long N, int num_tiles);           // depth chunks of one tile
-int device_sms();                                      // multiprocessors of the current device
 
 // Where a forward's colours come from: the features; the features rounded as
 // 4-bit records hold them; or records, which then stand in the place of the

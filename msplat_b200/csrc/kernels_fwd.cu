@@ -1396,7 +1396,7 @@ sort_flagged_tiles_kernel(const StepParams* __restrict__ P, const int* __restric
 }
 
 // SM count of the current device (148, the B200's, if the query fails).
-int device_sms()
+static int device_sms()
 {
     static std::once_flag once[kMaxDeviceSlots];
     static int sms[kMaxDeviceSlots];

@@ -156,6 +156,9 @@ __device__ __forceinline__ void color_of_record(const float* cam, const RawGauss
 // floats a thread: whole lines by way of shared memory took longer (13.1; 8 views
 // of 6M 232), the L2 joins the parts.  Degree 4 would spill at the other degrees' 64 registers.
 constexpr int one_view_blocks(int deg) { return deg == 4 ? 6 : 8; }
+// The B200's multiprocessors.  Blocks take tiles until none is left, so the number
+// is a matter of speed only; asking the runtime for it took 0.1 us of a call's 8.
+constexpr unsigned kSms = 148;
 template <int DEG, int USE, bool MASKED>
 __global__ void __launch_bounds__(kMxThreads, one_view_blocks(DEG))
 mx4_colors_one_kernel(int n, const float* __restrict__ means, const void* __restrict__ records,
@@ -326,7 +329,7 @@ int msplat_mx4_colors(int n, int degree, int degrees_to_use, const float* means3
         constexpr int d = D.value, u = U.value;
         const unsigned tiles = mx4_blocks(n);
         auto one = [&](auto kernel) {
-            const unsigned stay = std::min(tiles, (unsigned)(device_sms() * one_view_blocks(d)));
+            const unsigned stay = std::min(tiles, kSms * one_view_blocks(d));
             const Mx4Cam cam = {{cam_pos[0], cam_pos[1], cam_pos[2]}};
             rc = launch(who, kernel, stay, kMxThreads, st, n, means3d, records, cam, radii, colors);
         };
