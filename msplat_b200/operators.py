@@ -29,6 +29,8 @@ MAX_INT = 2**31 - 1                 # largest count that the C-ABI takes as an i
 # tensor that passes the checks.)
 _device_now = getattr(torch._C, "_cuda_getDevice", None)
 _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_F32 = np.dtype(np.float32)
+_bound = {}     # the library's functions by name, once called
 
 
 def _check(t, name: str, shape, dtype=torch.float32, device=None) -> None:
@@ -64,7 +66,7 @@ def _count(n: int, name: str) -> None:
 
 
 def _run(fn: str, device, *args) -> None:
-    call = getattr(_lib.load(), fn)
+    call = _bound.get(fn) or _bound.setdefault(fn, getattr(_lib.load(), fn))
     index = device.index
     if index == _device_now():
         rc = call(*args, _stream_of(index))
@@ -185,12 +187,13 @@ def mx4_unpack(records, degree: int, out=None):
 
 def _views(cam_pos):
     """Camera positions as C-ordered float32 (V, 3) in host bytes, and V."""
-    if isinstance(cam_pos, torch.Tensor):
+    if type(cam_pos) is not np.ndarray and isinstance(cam_pos, torch.Tensor):
         raise ValueError("cam_pos is host data: an array or nested list of shape (V, 3)")
-    cams = np.ascontiguousarray(cam_pos, dtype=np.float32)
-    if cams.ndim != 2 or cams.shape[1] != 3 or cams.shape[0] > MAX_VIEWS:
-        raise ValueError(f"cam_pos must have shape (V, 3), V <= {MAX_VIEWS}, not {cams.shape}")
-    return cams.tobytes(), cams.shape[0]
+    cams = np.asarray(cam_pos, _F32)
+    shape = cams.shape
+    if len(shape) != 2 or shape[1] != 3 or shape[0] > MAX_VIEWS:
+        raise ValueError(f"cam_pos must have shape (V, 3), V <= {MAX_VIEWS}, not {shape}")
+    return cams.tobytes(), shape[0]
 
 
 def _use(degrees_to_use, degree: int) -> int:

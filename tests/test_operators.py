@@ -177,6 +177,17 @@ def test_degrees_to_use_that_are_none(use):
         operators._use(use, 3)
 
 
+def test_camera_positions_as_bytes():
+    """C-ordered float32, whatever the array: its type, order and strides."""
+    want = np.arange(12, dtype=np.float32).reshape(4, 3)
+    wide = np.zeros((8, 6))
+    wide[::2, ::2] = want
+    for cams in (want, want.astype(np.float64), np.asfortranarray(want), want.tolist(), tuple(map(tuple, want)),
+                 wide[::2, ::2], want.astype(int)):
+        assert operators._views(cams) == (want.tobytes(), 4)
+    assert operators._views(want[:0]) == (b"", 0)
+
+
 def test_degrees_to_use():
     assert [operators._use(u, 3) for u in (None, 0, 3, np.int64(2), 1.0)] == [3, 0, 3, 2, 1]
 
